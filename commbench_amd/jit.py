@@ -46,8 +46,10 @@ def init_jit(overlay_root: Optional[str] = None, rocm_home: Optional[str] = None
              cache_dir: Optional[str] = None) -> None:
     """Sets where later compilations take their sources and compiler from.  A file of
     `overlay_root` named like a shipped kernel source (ep_layout.hip, ep_permute.hip, ep_combine.hip,
-    ep_abi.hip, ep_host.hip, ep_device.h) replaces it, as the reference's overlay replaces one
-    header; `rocm_home` is the toolchain root (hipcc under bin/)."""
+    ep_quantize.hip, ep_expert_matmul.hip, ep_few_tokens.hip, ep_abi.hip, ep_host.hip, ep_device.h)
+    replaces it, as the reference's overlay replaces one header; `rocm_home` is the toolchain root (hipcc
+    under bin/).  The quantisation and expert kernels hold no fixed shape: a library built for
+    one takes every shape in those calls."""
     if overlay_root is not None and not os.path.isdir(overlay_root):
         raise ValueError(f"overlay_root {overlay_root!r} is not a folder")
     _config.update(overlay_root=overlay_root, rocm_home=rocm_home, cache_dir=cache_dir)

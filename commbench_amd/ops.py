@@ -14,12 +14,16 @@ split into `num_ranks` partitions:
         -> (recv_x, recv_topk_idx, recv_topk_weights, handle)            format: one row per token
     combine_ranks(y, handle, recv_topk_weights) -> combined_x[, weights]  and destination rank
     dispatch_cached / pull_indices                                        pull form from a source map
+    rms_norm_quantize / quantize_rows / dequantize_rows                   8-bit payloads and back
+    grouped_matmul_int8                                                   an expert's product on its rows
+    moe_few_tokens; Buffer.moe_int8                                       the whole expert layer
     host_get_dispatch_layout / host_dispatch_layout / host_dispatch / host_dispatch_ranks /
     host_dispatch_cached / host_combine                                   numpy in, numpy out
 
 torch is used for device memory and streams only; all arithmetic runs in the HIP kernels of
 libmi_ep.so.  Nothing here falls back to torch ops or to the CPU.
 """
+import struct
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
@@ -34,6 +38,11 @@ ZERO_PAD_PAYLOAD = 1   # MI_EP_DISPATCH_ZERO_PAD_PAYLOAD
 BY_TOKEN = 2           # MI_EP_DISPATCH_BY_TOKEN
 BY_DESTINATION = 4     # MI_EP_DISPATCH_BY_DESTINATION
 STREAM_OUTPUT = 1      # MI_EP_COMBINE_STREAM_OUTPUT
+SILU_MUL = 1           # MI_EP_MATMUL_SILU_MUL
+QUANT_BLOCK = 128      # MI_EP_QUANT_BLOCK: columns that share an e4m3 scale
+QUANT_MAX_HIDDEN = 32768
+FEW_MAX_ROUTES = 1024  # MI_EP_FEW_MAX_ROUTES
+_QUANT_FORMATS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _SCHEDULE_FLAGS = {"auto": 0, "token": BY_TOKEN, "destination": BY_DESTINATION}
 
 
@@ -268,6 +277,24 @@ class Buffer:
             "mi_ep_dispatch_strided_scales")
         return recv_x, recv_scales, handle.recv_src_map, handle
 
+    def moe_int8(self, q: torch.Tensor, scales: torch.Tensor, topk_idx: torch.Tensor,
+                 topk_weights: Optional[torch.Tensor], w13: torch.Tensor, w13_scales: torch.Tensor, w2: torch.Tensor,
+                 w2_scales: torch.Tensor, bias=None, expert_alignment: int = 1) -> torch.Tensor:
+        """The whole expert layer on an int8 payload (rms_norm_quantize): dispatch, gate and up product with
+        silu(gate) * up, requantisation, down product, weighted combine (+ biases).  Weights as in
+        grouped_matmul_int8: w13 [experts, 2 * intermediate, hidden] (gate rows, then up rows), w2 [experts,
+        hidden, intermediate].  For a handful of tokens moe_few_tokens is the faster way."""
+        _require(q.dtype == torch.int8, "q must be int8 (rms_norm_quantize or quantize_rows)")
+        _require(scales is not None and scales.dim() == 2 and scales.shape[1] == 1, "scales must be float32 [num_tokens, 1]")
+        _require(w13.dim() == 3 and w2.dim() == 3 and w13.shape[0] == self.num_experts and w2.shape[0] == self.num_experts
+                 and w13.shape[1] == 2 * w2.shape[2] and w2.shape[1] == w13.shape[2] == q.shape[1],
+                 "w13 must be [experts, 2 * intermediate, hidden] and w2 [experts, hidden, intermediate]")
+        recv, recv_scales, _, h = self.dispatch(q, scales, topk_idx, topk_weights, expert_alignment)
+        act = grouped_matmul_int8(recv, recv_scales, w13, w13_scales, h.expert_offsets, h.num_tokens_per_expert, "silu_mul")
+        act_q, act_scales = quantize_rows(act, row_limit=h.expert_offsets[-1:])
+        y = grouped_matmul_int8(act_q, act_scales, w2, w2_scales, h.expert_offsets, h.num_tokens_per_expert)
+        return combine(y, h, topk_weights, bias)
+
 
 @dataclass
 class RankDispatchHandle:
@@ -482,6 +509,225 @@ def pull_indices(recv_src_map: torch.Tensor, tokens_per_source_rank: int,
     lib = _lib.load()
     _lib.check(lib.mi_ep_pull_indices(_ptr(recv_src_map), rows, tokens_per_source_rank, _ptr(out),
                                       _stream()), "mi_ep_pull_indices")
+    return out
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point on the current stream of the tensors' device, whichever device is current."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if code != 0:
+        _lib.check(code, name)
+
+
+def _quant_format(quant: str, width: int):
+    _require(quant in _QUANT_FORMATS, 'quant must be "int8" or "e4m3"')
+    _require(width > 0 and width % 8 == 0 and width <= QUANT_MAX_HIDDEN,
+             f"hidden must be a multiple of 8, at most {QUANT_MAX_HIDDEN}")
+    if quant == "e4m3":
+        _require(width % QUANT_BLOCK == 0, f"hidden must be a multiple of {QUANT_BLOCK} for e4m3")
+        return (*_QUANT_FORMATS[quant], width // QUANT_BLOCK)
+    return (*_QUANT_FORMATS[quant], 1)
+
+
+def _check_rows(x: torch.Tensor, name: str, device: Optional[torch.device] = None) -> None:
+    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1)
+             and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0)) and x.data_ptr() % 16 == 0,
+             f"{name} must be a bf16 [rows, hidden] GPU tensor of 16-byte aligned rows")
+    _require(device is None or x.device == device, f"{name} must live on the device of x")
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _check_row_limit(row_limit: Optional[torch.Tensor], device: torch.device) -> None:
+    _require(row_limit is None or (row_limit.dtype == torch.int32 and row_limit.numel() == 1
+                                   and row_limit.device == device),
+             "row_limit must be one int32 on the rows' device")
+
+
+def _empty_scales(rows: int, groups: int, device: torch.device, column_major: bool) -> torch.Tensor:
+    if column_major:
+        return torch.empty((groups, rows), dtype=torch.float32, device=device).t()
+    return torch.empty((rows, groups), dtype=torch.float32, device=device)
+
+
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                      residual: Optional[torch.Tensor] = None, quant: str = "int8", normed: bool = False,
+                      update_residual: bool = False, column_major_scales: bool = False):
+    """The root-mean-square norm of x (+ residual) as an 8-bit dispatch payload, in one pass:
+    h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight, q = round(y / scale).
+
+    `quant` is "int8" (a scale for each row, max|y| / 127) or "e4m3" (float8_e4m3fn, a scale for each 128
+    columns, max|y| / 448); scales come as float32 [rows, groups], what dispatch takes.  Returns (q, scales),
+    then the new residual stream bf16(h) when `residual` is given (written over it with
+    `update_residual`), then bf16(y) with `normed`.  x and residual may be views with padded rows."""
+    _check_rows(x, "x")
+    T, H = x.shape
+    fmt, dtype, groups = _quant_format(quant, H)
+    dev = x.device
+    _require(weight.dtype == torch.bfloat16 and weight.dim() == 1 and weight.shape[0] == H and weight.is_contiguous()
+             and weight.device == dev and weight.data_ptr() % 16 == 0, "weight must be contiguous bf16 [hidden] on the device of x")
+    _require(0.0 <= eps < float("inf"), "eps must be finite and not negative")
+    out_residual = None
+    if residual is not None:
+        _check_rows(residual, "residual", dev)
+        _require(residual.shape == x.shape, "residual must have the shape of x")
+        _require(not update_residual or residual.is_contiguous(), "a residual updated in place must be contiguous")
+        out_residual = residual if update_residual else torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+    else:
+        _require(not update_residual, "update_residual needs a residual")
+    q = torch.empty((T, H), dtype=dtype, device=dev)
+    scales = _empty_scales(T, groups, dev, column_major_scales)
+    out_normed = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if normed else None
+    _launch(dev, "mi_ep_rms_norm_quantize", x.data_ptr(), _row_stride(x), _ptr(residual),
+            _row_stride(residual) if residual is not None else 0, weight.data_ptr(),
+            struct.unpack("<I", struct.pack("<f", eps))[0], T, H, fmt, q.data_ptr(), scales.data_ptr(), *_scale_strides(scales),
+            _ptr(out_residual), _ptr(out_normed))
+    return tuple(t for t in (q, scales, out_residual, out_normed) if t is not None)
+
+
+def _scale_strides(scales: torch.Tensor) -> Tuple[int, int]:
+    return scales.stride(0), scales.stride(1)
+
+
+def quantize_rows(x: torch.Tensor, quant: str = "int8", row_limit: Optional[torch.Tensor] = None,
+                  column_major_scales: bool = False):
+    """Rows of bf16 to 8 bits with scales, as rms_norm_quantize makes them: (q, scales).  With `row_limit`
+    (one int32 on the device, e.g. handle.expert_offsets[-1:]) rows at and beyond it are left as they
+    were: what a receive buffer holds behind its last row is not touched."""
+    _check_rows(x, "x")
+    rows, H = x.shape
+    fmt, dtype, groups = _quant_format(quant, H)
+    _check_row_limit(row_limit, x.device)
+    q = torch.empty((rows, H), dtype=dtype, device=x.device)
+    scales = _empty_scales(rows, groups, x.device, column_major_scales)
+    _launch(x.device, "mi_ep_quantize_rows", x.data_ptr(), _row_stride(x), _ptr(row_limit), rows, H, fmt, q.data_ptr(),
+            scales.data_ptr(), *_scale_strides(scales))
+    return q, scales
+
+
+def dequantize_rows(q: torch.Tensor, scales: torch.Tensor, row_limit: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16(q * scale) of int8 rows with a scale each or float8_e4m3fn rows with a scale for each 128
+    columns: an 8-bit payload (x, or recv_x after dispatch) for experts that compute in bf16.  `scales` may
+    be any 2-D float32 view."""
+    _require(q.is_cuda and q.dim() == 2 and q.is_contiguous() and q.dtype in (torch.int8, torch.float8_e4m3fn),
+             "q must be a contiguous int8 or float8_e4m3fn [rows, hidden] GPU tensor")
+    rows, H = q.shape
+    fmt, _, groups = _quant_format("int8" if q.dtype == torch.int8 else "e4m3", H)
+    _require(scales.dtype == torch.float32 and tuple(scales.shape) == (rows, groups) and scales.device == q.device
+             and min(scales.stride()) >= 0, "scales must be a float32 [rows, groups] tensor or view on the device of q")
+    _check_row_limit(row_limit, q.device)
+    out = torch.empty((rows, H), dtype=torch.bfloat16, device=q.device)
+    _launch(q.device, "mi_ep_dequantize_rows", q.data_ptr(), scales.data_ptr(), *_scale_strides(scales), _ptr(row_limit),
+            rows, H, fmt, out.data_ptr())
+    return out
+
+
+def _check_int8_weight(b: torch.Tensor, b_scales: torch.Tensor, device: torch.device, name: str) -> None:
+    _require(b.dtype == torch.int8 and b.dim() == 3 and b.is_contiguous() and b.device == device
+             and b.data_ptr() % 16 == 0, f"{name} must be contiguous int8 [experts, out, in] on the device of the rows")
+    _require(b_scales.dtype == torch.float32 and b_scales.is_contiguous() and b_scales.shape == b.shape[:2]
+             and b_scales.device == device, f"{name}'s scales must be contiguous float32 [experts, out] on its device")
+
+
+def grouped_matmul_int8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+                        expert_offsets: Optional[torch.Tensor] = None,
+                        num_tokens_per_expert: Optional[torch.Tensor] = None, activation: Optional[str] = None):
+    """The experts' product on dispatched rows: bf16(a_scale[m] * b_scale[e, n] * sum_k a[m, k] b[e, n, k]) for the
+    rows m of every expert e, summed in 32-bit integers.
+
+    a is int8 [rows, in] with one float32 scale for each row ([rows] or [rows, 1], any stride: recv_x and
+    recv_scales of an int8 dispatch), b int8 [experts, out, in] with scales [experts, out];
+    `expert_offsets` and `num_tokens_per_expert` are the layout's (without the counts pad rows are computed
+    too; without both, one expert owns all rows: a plain product).  With activation="silu_mul", b holds
+    out / 2 gate and out / 2 up channels and the result is silu(gate) * up.  Rows of no expert (pads, rows
+    behind the last segment) are not written."""
+    _require(a.is_cuda and a.dtype == torch.int8 and a.dim() == 2 and a.is_contiguous() and a.data_ptr() % 16 == 0,
+             "a must be a contiguous int8 [rows, in] GPU tensor")
+    dev = a.device
+    _check_int8_weight(b, b_scales, dev, "b")
+    rows, k = a.shape
+    experts, n, _ = b.shape
+    _require(b.shape[2] == k, "a and b differ in their inner size")
+    _require(0 < k < 131072 and k % 16 == 0, "the inner size must be a multiple of 16 below 131072")
+    _require(activation in (None, "silu_mul"), 'activation must be None or "silu_mul"')
+    _require(n > 0 and n % (16 if activation else 8) == 0, "the output size must be a multiple of 8 (16 with silu_mul)")
+    _require(0 < experts <= MAX_EXPERTS, f"the number of experts must be in [1, {MAX_EXPERTS}]")
+    _require(a_scales.dtype == torch.float32 and a_scales.device == dev and a_scales.shape[0] == rows
+             and (a_scales.dim() == 1 or (a_scales.dim() == 2 and a_scales.shape[1] == 1)) and a_scales.stride(0) >= 0,
+             "a_scales must be float32 [rows] or [rows, 1] on the device of a")
+    if expert_offsets is None:
+        _require(experts == 1 and num_tokens_per_expert is None, "several experts need expert_offsets")
+    else:
+        _require(expert_offsets.dtype == torch.int32 and expert_offsets.is_contiguous() and expert_offsets.device == dev
+                 and tuple(expert_offsets.shape) == (experts + 1,), "expert_offsets must be contiguous int32 [experts + 1]")
+        _require(num_tokens_per_expert is None
+                 or (num_tokens_per_expert.dtype == torch.int32 and num_tokens_per_expert.is_contiguous()
+                     and num_tokens_per_expert.device == dev and tuple(num_tokens_per_expert.shape) == (experts,)),
+                 "num_tokens_per_expert must be contiguous int32 [experts]")
+    out = torch.empty((rows, n // 2 if activation else n), dtype=torch.bfloat16, device=dev)
+    _launch(dev, "mi_ep_grouped_matmul_int8", a.data_ptr(), a_scales.data_ptr(), a_scales.stride(0), b.data_ptr(),
+            b_scales.data_ptr(), _ptr(expert_offsets), _ptr(num_tokens_per_expert), rows, experts, n, k, out.data_ptr(),
+            SILU_MUL if activation else 0)
+    return out
+
+
+def moe_few_tokens(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: Optional[torch.Tensor], w13: torch.Tensor,
+                   w2: torch.Tensor, w13_scales: Optional[torch.Tensor] = None, w2_scales: Optional[torch.Tensor] = None,
+                   bias: Union[None, torch.Tensor, Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]] = None):
+    """The whole expert layer for a few tokens (num_tokens * num_topk <= 1024) in two launches:
+    out[t] = sum_k w[t,k] * W2[e] (silu(Wgate[e] x[t]) * (Wup[e] x[t])) (+ biases), e = topk_idx[t,k].
+
+    x is bf16 [tokens, hidden]; w13 [experts, 2 * intermediate, hidden] holds the gate rows, then the up
+    rows, w2 is [experts, hidden, intermediate]; both bf16, or int8 with float32 scales [experts, rows].
+    topk_idx, topk_weights (None: a plain sum) and bias as in dispatch and combine; a token whose slots are all
+    masked gets its biases.  With many tokens Buffer.moe_int8 is the faster way."""
+    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0,
+             "x must be a contiguous bf16 [num_tokens, hidden] GPU tensor")
+    dev = x.device
+    T, H = x.shape
+    _require(topk_idx.dtype == torch.int64 and topk_idx.dim() == 2 and topk_idx.is_contiguous()
+             and topk_idx.shape[0] == T and topk_idx.device == dev,
+             "topk_idx must be a contiguous int64 [num_tokens, num_topk] tensor on the device of x")
+    K = topk_idx.shape[1]
+    _require(0 < K <= MAX_TOPK, f"num_topk must be in [1, {MAX_TOPK}]")
+    _require(T * K <= FEW_MAX_ROUTES, f"num_tokens * num_topk must be at most {FEW_MAX_ROUTES}")
+    _require(topk_weights is None or (topk_weights.dtype == torch.float32 and topk_weights.is_contiguous()
+                                      and topk_weights.shape == topk_idx.shape and topk_weights.device == dev),
+             "topk_weights must be contiguous float32 [num_tokens, num_topk]")
+    _require(w13.dim() == 3 and w2.dim() == 3 and w13.shape[1] % 2 == 0, "w13 and w2 must be [experts, out, in]")
+    E, I = w13.shape[0], w13.shape[1] // 2
+    _require(0 < E <= MAX_EXPERTS, f"the number of experts must be in [1, {MAX_EXPERTS}]")
+    _require(tuple(w13.shape) == (E, 2 * I, H) and tuple(w2.shape) == (E, H, I),
+             "w13 must be [experts, 2 * intermediate, hidden] and w2 [experts, hidden, intermediate]")
+    _require(0 < H <= 65536 and 0 < I <= 65536 and H % 16 == 0 and I % 16 == 0,
+             "hidden and intermediate must be multiples of 16, at most 65536")
+    _require((w13_scales is None) == (w2_scales is None), "both weights have scales or neither has")
+    if w13_scales is not None:
+        _check_int8_weight(w13, w13_scales, dev, "w13")
+        _check_int8_weight(w2, w2_scales, dev, "w2")
+    else:
+        for w, name in ((w13, "w13"), (w2, "w2")):
+            _require(w.dtype == torch.bfloat16 and w.is_contiguous() and w.device == dev and w.data_ptr() % 16 == 0,
+                     f"{name} must be contiguous bf16 (or int8 with scales) on the device of x")
+    bias_0, bias_1 = bias if isinstance(bias, tuple) else (bias, None)
+    for b in (bias_0, bias_1):
+        _require(b is None or (b.dtype == torch.bfloat16 and b.is_contiguous() and tuple(b.shape) == (T, H)
+                               and b.device == dev and b.data_ptr() % 16 == 0),
+                 "bias must be contiguous bf16 [num_tokens, hidden]")
+    out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+    # A workspace of the call's own: calls on other streams, and captured graphs, never share one.
+    nbytes = _lib.load().mi_ep_moe_few_tokens_workspace_bytes(T, K, I)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "mi_ep_moe_few_tokens", x.data_ptr(), topk_idx.data_ptr(), _ptr(topk_weights), w13.data_ptr(),
+            _ptr(w13_scales), w2.data_ptr(), _ptr(w2_scales), _ptr(bias_0), _ptr(bias_1), T, K, E, H, I, out.data_ptr(),
+            work.data_ptr(), nbytes)
     return out
 
 

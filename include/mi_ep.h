@@ -383,6 +383,95 @@ int mi_ep_combine(const void* y, int num_rows, const int* slot_map, const float*
                   int flags, void* stream);
 
 /*
+ * Rows to 8 bits: what a dispatch sends when its payload is quantised, made where the row is made.
+ *   h = x + residual;  y = h / sqrt(mean(h^2) + epsilon) * weight          (mi_ep_rms_norm_quantize)
+ *   y = x                                                                  (mi_ep_quantize_rows)
+ *   scale = max|y| / qmax, 1 where that is 0;  q = round(y / scale), ties to even
+ * all in fp32 from the bf16 inputs, one rounding to the codes.
+ *   format       MI_EP_QUANT_INT8_ROW: int8, qmax 127, one scale per row.
+ *                MI_EP_QUANT_E4M3_BLOCK: e4m3 (the OCP form), qmax 448, one scale per 128 columns
+ *                (hidden % 128 == 0).
+ *   x, residual  bf16 [num_rows, hidden], rows x_row_stride / residual_row_stride elements apart (at
+ *                least hidden, multiples of 8); residual may be NULL
+ *   weight       bf16 [hidden]
+ *   epsilon_bits the fp32 epsilon (finite, not negative) as its IEEE-754 bits: every value of this ABI
+ *                that is not a pointer is an integer
+ *   row_limit    NULL, or one int32 of device memory: rows at and beyond it are left as they were
+ *                (expert_offsets + num_experts of a layout: the rows a dispatch has filled)
+ *   q            8-bit [num_rows, hidden], 8-byte aligned
+ *   scales       float, element j of row r at scales[r * scales_row_stride + j * scales_hidden_stride],
+ *                the strides mi_ep_dispatch_strided_scales takes; written scales may not share a place
+ *   residual_out bf16 [num_rows, hidden] or NULL: h rounded once.  It may be residual or x themselves (with a
+ *                row stride of hidden); needs residual
+ *   normed       bf16 [num_rows, hidden] or NULL: y rounded once (for a router or a bf16 branch)
+ * A row (block) that holds an infinity or a NaN gets a NaN scale and reads back as NaN throughout.
+ * hidden % 8 == 0, hidden <= 32768; bf16 pointers 16-byte aligned.  Outputs must not overlap inputs otherwise.
+ * mi_ep_dequantize_rows reads them back: out = bf16(q * scale).
+ */
+#define MI_EP_QUANT_INT8_ROW 0
+#define MI_EP_QUANT_E4M3_BLOCK 1
+#define MI_EP_QUANT_BLOCK 128
+#define MI_EP_QUANT_MAX_HIDDEN 32768
+int mi_ep_rms_norm_quantize(const void* x, long long x_row_stride, const void* residual,
+                            long long residual_row_stride, const void* weight, unsigned int epsilon_bits,
+                            int num_rows, int hidden, int format, void* q, float* scales,
+                            long long scales_row_stride, long long scales_hidden_stride, void* residual_out,
+                            void* normed, void* stream);
+int mi_ep_quantize_rows(const void* x, long long x_row_stride, const int* row_limit, int num_rows, int hidden,
+                        int format, void* q, float* scales, long long scales_row_stride,
+                        long long scales_hidden_stride, void* stream);
+int mi_ep_dequantize_rows(const void* q, const float* scales, long long scales_row_stride,
+                          long long scales_hidden_stride, const int* row_limit, int num_rows, int hidden,
+                          int format, void* out, void* stream);
+
+/*
+ * The experts' product on the rows a dispatch has put together, int8 by int8 with a scale for every
+ * row and every output channel, 32-bit integer sums:
+ *   c[m, n] = a_scales[m] * b_scales[e, n] * sum_k a[m, k] * b[e, n, k]    for the rows m of expert e
+ *   out[m, :] = bf16(c[m, :]), or with MI_EP_MATMUL_SILU_MUL, out_features = 2 I,
+ *   out[m, i] = bf16(silu(c[m, i]) * c[m, I + i])                          (gate rows of b, then up rows)
+ *   a            int8 [num_rows, in_features] (recv_x of an int8 dispatch); a_scales: one float per row,
+ *                a_scales_row_stride apart (recv_scales with num_scales = 1)
+ *   b, b_scales  int8 [num_experts, out_features, in_features], float [num_experts, out_features]
+ *   expert_offsets, num_tokens_per_expert   from the layout: the rows of expert e are
+ *                expert_offsets[e] .. + num_tokens_per_expert[e] (to expert_offsets[e + 1] when the counts are
+ *                NULL: pad rows are computed too).  Both NULL with num_experts == 1: one expert owns all rows.
+ *   out          bf16 [num_rows, out_features or I]; rows that belong to no expert are left as they were
+ * in_features % 16 == 0 and below 131072, out_features % 8 == 0 (% 16 with SILU_MUL), num_experts <= 1024; a,
+ * b, out 16-byte aligned.  num_rows is the capacity: segments are clamped to it.
+ */
+#define MI_EP_MATMUL_SILU_MUL 1
+int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_scales_row_stride, const void* b,
+                              const float* b_scales, const int* expert_offsets,
+                              const int* num_tokens_per_expert, int num_rows, int num_experts, int out_features,
+                              int in_features, void* out, int flags, void* stream);
+
+/*
+ * The whole expert layer for a few tokens, in two launches and without moving a row:
+ *   combined_x[t] = bf16( sum_k w[t,k] * W2[e] (silu(Wgate[e] x[t]) * (Wup[e] x[t])) + bias_0[t] + bias_1[t] ),
+ *   e = topk_idx[t, k]; slots outside [0, num_experts) are no routes, a token without routes gets its biases
+ * (zeros without).  It reads the weights of the experts that the tokens met, once; with many tokens dispatch, the
+ * products above and combine are the faster way.
+ *   x            bf16 [num_tokens, hidden]
+ *   w13, w2      [num_experts, 2 * intermediate, hidden] (gate rows, then up rows), [num_experts, hidden,
+ *                intermediate]: bf16 with both scales NULL, or int8 with w13_scales float [num_experts, 2 *
+ *                intermediate] and w2_scales float [num_experts, hidden], one per output channel
+ *   topk_weights float [num_tokens, num_topk] or NULL: a plain sum
+ *   workspace    mi_ep_moe_few_tokens_workspace_bytes bytes, 16-byte aligned, no initialisation; calls that
+ *                share one must not overlap in time
+ * Sums are fp32 in an order that depends on the shapes alone; the activation between the two products is
+ * rounded to bf16.  num_tokens * num_topk <= MI_EP_FEW_MAX_ROUTES; hidden % 16 == 0, intermediate % 16 == 0, both
+ * at most 65536; x, w13, w2, biases and combined_x 16-byte aligned.
+ */
+#define MI_EP_FEW_MAX_ROUTES 1024
+size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int intermediate);
+int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* topk_weights, const void* w13,
+                         const float* w13_scales, const void* w2, const float* w2_scales, const void* bias_0,
+                         const void* bias_1, int num_tokens, int num_topk, int num_experts, int hidden,
+                         int intermediate, void* combined_x, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
  * Host-pointer twins: the same operations with every pointer in ordinary host memory.  Each call
  * allocates device buffers, copies inputs over, runs the kernels above on the null stream, copies
  * the outputs back and returns after synchronising; errors as above.  They serve callers without a
