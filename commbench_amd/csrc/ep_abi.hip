@@ -671,7 +671,7 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
   // |a * b| <= 2^14: 2^17 of them are the most whose sum is sure to fit 32 bits.
   if (in_features <= 0 || in_features % 16 != 0 || in_features >= (1 << 17)) return MI_EP_EINVAL;
   if (out_features <= 0 || out_features % (silu_mul ? 16 : 8) != 0 || out_features > (1 << 20)) return MI_EP_EINVAL;
-  if (a_scales_row_stride < 0) return MI_EP_EINVAL;
+  if (a_scales_row_stride < 0 || a_scales_row_stride > (1 << 20)) return MI_EP_EINVAL;  // a tile's scales lie within 2^30 bytes
   if (expert_offsets == nullptr && (num_experts != 1 || num_tokens_per_expert != nullptr)) return MI_EP_EINVAL;
   if (!aligned16(a) || !aligned16(b) || !aligned16(out)) return MI_EP_EINVAL;
   if (num_rows > 0 && (a == nullptr || a_scales == nullptr || b == nullptr || b_scales == nullptr || out == nullptr))

@@ -3,6 +3,7 @@
 //   c[m, n] = a_scale[m] * b_scale[e, n] * sum_k a[m, k] * b[e, n, k]     rows m of expert e's segment
 //   out = bf16(c)   or, gate and up in one product,   out[m, i] = bf16(silu(c[m, i]) * c[m, I + i])
 // The sum over k is exact in 32-bit integers (|a|, |b| <= 128 and k < 2^17).
+#include <cstdlib>
 #include "ep_device.h"
 
 namespace mi_ep {
@@ -10,128 +11,530 @@ namespace {
 
 typedef int int4v __attribute__((ext_vector_type(4)));
 
-constexpr int kTileM = 64, kTileN = 64, kStepK = 64;
-constexpr int kPitch = kStepK + 16;  // bytes between LDS rows: 16-byte reads of 16 rows meet different banks
+constexpr int kBigK = 64;                                      // bytes of k in a stage
+constexpr int kChunkBytes = 1024;                              // what one load instruction of a wave moves
+constexpr int kOutside = static_cast<int>(0x80000000u);        // an offset beyond every descriptor
+
+typedef int int16v __attribute__((ext_vector_type(16)));
+
+struct Segment {
+  int first, rows;
+};
+__device__ __forceinline__ Segment segment_of(const ExpertMatmulArgs& a, int e) {
+  long long lo = 0, hi = a.num_rows;
+  if (a.expert_offsets != nullptr) {
+    lo = a.expert_offsets[e];
+    hi = a.num_tokens_per_expert != nullptr ? lo + a.num_tokens_per_expert[e] : a.expert_offsets[e + 1];
+  }
+  if (lo < 0) lo = 0;
+  if (hi > a.num_rows) hi = a.num_rows;
+  return hi > lo ? Segment{static_cast<int>(lo), static_cast<int>(hi - lo)} : Segment{0, 0};
+}
+
+// 64 lanes x 16 bytes from global memory to 1 KiB of LDS at `lds` (wave-uniform), not waited for.  In
+// assembly because the compiler would wait for every load before the next LDS read of any address; the
+// waits are written at the end of each step instead.  A lane whose offset lies outside the descriptor moves
+// zeros and makes no memory request.
+__device__ __forceinline__ void load_to_lds(int4v descriptor, int lds, int lane_offset, int scalar_offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(lds), "v"(lane_offset), "s"(descriptor), "s"(scalar_offset)
+               : "memory");
+}
+__device__ __forceinline__ void load_word_to_lds(int4v descriptor, int lds, int lane_offset) {  // 4 bytes a lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(lane_offset), "s"(descriptor)
+               : "memory");
+}
+__device__ __forceinline__ int4v descriptor_of(const void* base, int bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  return int4v{__builtin_amdgcn_readfirstlane(static_cast<int>(at)),
+               __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32) & 0xffff), __builtin_amdgcn_readfirstlane(bytes),
+               kRawBufferFormat};
+}
+
+// Two fp32 values as packed bf16, rounded to nearest even in one instruction.
+__device__ __forceinline__ uint32_t to_bf16_pair(float lo, float hi) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  union {
+    bf16x2 b;
+    uint32_t u;
+  } out;
+  out.b = __builtin_convertvector((float2v{lo, hi}), bf16x2);
+  return out.u;
+}
+
+// The byte address in LDS of a pointer into it.
+__device__ __forceinline__ int lds_address(const unsigned char* p) {
+  return static_cast<int>((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p);
+}
+
+// v / (1 + exp(-v)); the reciprocal instruction is off by one unit in the last place at most.
+__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+
+// A lane's part in the loads and reads of a stage.  A stage holds rows of 64 bytes, two to a 128-byte line; the
+// line's eight 16-byte pieces are permuted by exclusive or with the line number, so that 8 lanes reading one
+// piece of 8 rows meet all banks.  A load instruction fills 16 rows in order; lane l of it fetches the piece
+// that belongs at l.
+struct Place {
+  int piece, row, read_at;
+  __device__ __forceinline__ explicit Place(int lane) {
+    const int logical = (lane & 7) ^ (lane >> 3), r = lane & 31;
+    piece = (logical & 3) * 16;
+    row = (lane >> 3) * 2 + (logical >> 2);
+    read_at = (r >> 1) * 128 + ((((r & 1) * 4 + (lane >> 5)) ^ ((r >> 1) & 7)) * 16);
+  }
+};
+
+
+// ---- small tiles: 64 rows by 64 columns, for problems of few tiles --------------------------------------
+constexpr int kTileM = 64, kTileN = 64;
+constexpr int kSmallThreads = 256;
 
 struct RowTile {
   int expert, first, rows;  // rows [first, first + rows) of a and out; rows == 0: no such tile
 };
 
 // The `index`-th tile of up to kTileM rows, the experts' segments cut into tiles one after the other.
-// Segments are clamped to [0, num_rows), whatever the tables hold.
 __device__ __forceinline__ RowTile find_row_tile(const ExpertMatmulArgs& a, int index) {
-  __shared__ int wave_tiles[4];
+  if (a.expert_offsets == nullptr) {
+    const int left = a.num_rows - index * kTileM;
+    return RowTile{0, index * kTileM, left < 0 ? 0 : left < kTileM ? left : kTileM};
+  }
+  __shared__ int wave_tiles[kSmallThreads / kWave];
   __shared__ RowTile found;
   const int t = static_cast<int>(threadIdx.x);
-  const int per = (a.num_experts + 255) / 256;
+  const int per = (a.num_experts + kSmallThreads - 1) / kSmallThreads;
   if (t == 0) found = RowTile{0, 0, 0};
+  Segment segments[kMaxExperts / kSmallThreads];
   int mine = 0;
-  const auto segment = [&](int e, int* first) {
-    long long lo = 0, hi = a.num_rows;
-    if (a.expert_offsets != nullptr) {
-      lo = a.expert_offsets[e];
-      hi = a.num_tokens_per_expert != nullptr ? lo + a.num_tokens_per_expert[e] : a.expert_offsets[e + 1];
-    }
-    if (lo < 0) lo = 0;
-    if (hi > a.num_rows) hi = a.num_rows;
-    *first = static_cast<int>(lo);
-    return hi > lo ? static_cast<int>(hi - lo) : 0;
-  };
-  for (int j = 0; j < per; ++j) {
+#pragma unroll
+  for (int j = 0; j < kMaxExperts / kSmallThreads; ++j) {
     const int e = t * per + j;
-    int first;
-    if (e < a.num_experts) mine += (segment(e, &first) + kTileM - 1) / kTileM;
+    segments[j] = j < per && e < a.num_experts ? segment_of(a, e) : Segment{0, 0};
+    mine += (segments[j].rows + kTileM - 1) / kTileM;
   }
   const int upto = wave_inclusive_scan(mine);
   if (lane_id() == kWave - 1) wave_tiles[t >> 6] = upto;
   __syncthreads();
   int before = upto - mine;
   for (int w = 0; w < (t >> 6); ++w) before += wave_tiles[w];
-  if (index >= before && index < before + mine) {
-    for (int j = 0; j < per; ++j) {
-      const int e = t * per + j;
-      int first = 0;
-      const int rows = e < a.num_experts ? segment(e, &first) : 0;
-      const int tiles = (rows + kTileM - 1) / kTileM;
-      if (index >= before && index < before + tiles) {
-        const int skip = (index - before) * kTileM;
-        found = RowTile{e, first + skip, rows - skip < kTileM ? rows - skip : kTileM};
-      }
-      before += tiles;
+#pragma unroll
+  for (int j = 0; j < kMaxExperts / kSmallThreads; ++j) {
+    const int tiles = (segments[j].rows + kTileM - 1) / kTileM;
+    if (index >= before && index < before + tiles) {
+      const int skip = (index - before) * kTileM;
+      found = RowTile{t * per + j, segments[j].first + skip,
+                      segments[j].rows - skip < kTileM ? segments[j].rows - skip : kTileM};
     }
+    before += tiles;
   }
   __syncthreads();
-  return found;
+  return RowTile{__builtin_amdgcn_readfirstlane(found.expert), __builtin_amdgcn_readfirstlane(found.first),
+                 __builtin_amdgcn_readfirstlane(found.rows)};
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
-
-// One workgroup: 64 rows by 64 output columns (with kSilu the 64 gate and the 64 up channels of those
-// columns).  Wave w owns 16 output columns.
+// Wave (mw, nw) owns 32 rows and 32 columns (with kSilu their gate and their up channels).
 template <bool kSilu>
-__global__ __launch_bounds__(256) void ep_expert_matmul_kernel(const ExpertMatmulArgs a) {
+__global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(const ExpertMatmulArgs a) {
   constexpr int kSets = kSilu ? 2 : 1;
-  __shared__ __align__(16) unsigned char stage_a[kTileM * kPitch];
-  __shared__ __align__(16) unsigned char stage_b[kSets * kTileN * kPitch];
+  constexpr int kRing = 6;
+  constexpr int kABytes = kTileM * kBigK, kStage = kABytes + kSets * kTileN * kBigK;
+  constexpr int kLoads = 1 + kSets;  // of a wave for a stage
+  __shared__ __align__(1024) unsigned char ring[kRing * kStage];
   const RowTile tile = find_row_tile(a, static_cast<int>(blockIdx.y));
-  if (tile.rows == 0) return;
-  const int out_columns = kSilu ? a.out_features / 2 : a.out_features;
+  if (tile.rows <= 0) return;
+  const int K = a.in_features;
+  const int columns = kSilu ? a.out_features / 2 : a.out_features;
   const int n0 = static_cast<int>(blockIdx.x) * kTileN;
-  const int t = static_cast<int>(threadIdx.x), lane = lane_id(), wave = t >> 6;
-  const int load_row = t >> 2, load_k = (t & 3) * 16;
+  const int lane = lane_id(), r = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int mw = wave & 1, nw = wave >> 1;
+  const int steps = (K + kBigK - 1) / kBigK;
+  const Place at(lane);
+  const int b_rows = columns - n0 < kTileN ? columns - n0 : kTileN;
+  const size_t channel = static_cast<size_t>(tile.expert) * a.out_features + n0;
+  const int4v desc_a = descriptor_of(a.a + static_cast<size_t>(tile.first) * K, tile.rows * K);
+  const int4v desc_b = descriptor_of(a.b + channel * K, b_rows * K);
+  const int4v desc_up = kSilu ? descriptor_of(a.b + (channel + columns) * K, b_rows * K) : desc_b;
+  const int offset = (wave * 16 + at.row) * K + at.piece;
+  const int ring_base = lds_address(ring);
+  int load_slot = 0;
+  const auto load_stage = [&](int step) {  // steps behind the last load nothing, but count
+    const int k0 = step < steps ? step * kBigK : 0;
+    const int from = step * kBigK + at.piece < K ? offset : kOutside;
+    const int to = ring_base + load_slot * kStage + wave * kChunkBytes;
+    load_to_lds(desc_a, to, from, k0);
+    load_to_lds(desc_b, to + kABytes, from, k0);
+    if constexpr (kSilu) load_to_lds(desc_up, to + kABytes + kTileN * kBigK, from, k0);
+    load_slot = load_slot + 1 == kRing ? 0 : load_slot + 1;
+  };
+#pragma unroll
+  for (int s = 0; s < kRing - 1; ++s) load_stage(s);
 
-  const unsigned char* a_row = a.a + static_cast<size_t>(tile.first + (load_row < tile.rows ? load_row : 0)) * a.in_features;
-  const int n_row = n0 + load_row < out_columns ? n0 + load_row : out_columns - 1;
-  const unsigned char* b_row =
-      a.b + (static_cast<size_t>(tile.expert) * a.out_features + n_row) * a.in_features;
-
-  int4v acc[kSets][kTileM / 16];
+  int16v acc[kSets];
 #pragma unroll
-  for (int s = 0; s < kSets; ++s)
+  for (int s = 0; s < kSets; ++s) acc[s] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+  int slot = 0;
+  for (int step = 0; step < steps; ++step) {
+    // Stage step is in, and every wave has left the stage before it, whose place the next load takes.
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((kRing - 2) * kLoads) : "memory");
+    load_stage(step + kRing - 1);
+    const unsigned char* stage = ring + slot * kStage;
 #pragma unroll
-    for (int m = 0; m < kTileM / 16; ++m) acc[s][m] = int4v{0, 0, 0, 0};
-
-  for (int k0 = 0; k0 < a.in_features; k0 += kStepK) {
-    const bool inside = k0 + load_k < a.in_features;
-    const vec16 zero = {0, 0, 0, 0};
-    *reinterpret_cast<vec16*>(stage_a + load_row * kPitch + load_k) =
-        inside ? *reinterpret_cast<const vec16*>(a_row + k0 + load_k) : zero;
+    for (int half = 0; half < 2; ++half) {
+      const unsigned char* base = stage + (at.read_at ^ (half * 32));
+      const int4v rows = *reinterpret_cast<const int4v*>(base + mw * 2048);
 #pragma unroll
-    for (int s = 0; s < kSets; ++s)
-      *reinterpret_cast<vec16*>(stage_b + (s * kTileN + load_row) * kPitch + load_k) =
-          inside ? *reinterpret_cast<const vec16*>(b_row + static_cast<size_t>(s) * out_columns * a.in_features + k0 + load_k)
-                 : zero;
-    __syncthreads();
-    int4v w[kSets];
-#pragma unroll
-    for (int s = 0; s < kSets; ++s)
-      w[s] = *reinterpret_cast<const int4v*>(stage_b + (s * kTileN + wave * 16 + (lane & 15)) * kPitch + (lane >> 4) * 16);
-#pragma unroll
-    for (int m = 0; m < kTileM / 16; ++m) {
-      const int4v x = *reinterpret_cast<const int4v*>(stage_a + (m * 16 + (lane & 15)) * kPitch + (lane >> 4) * 16);
-#pragma unroll
-      for (int s = 0; s < kSets; ++s) acc[s][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[s], x, acc[s][m], 0, 0, 0);
+      for (int s = 0; s < kSets; ++s) {
+        const int4v channels = *reinterpret_cast<const int4v*>(base + kABytes + s * kTileN * kBigK + nw * 2048);
+        acc[s] = __builtin_amdgcn_mfma_i32_32x32x32_i8(channels, rows, acc[s], 0, 0, 0);
+      }
     }
-    __syncthreads();
+    slot = slot + 1 == kRing ? 0 : slot + 1;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the workgroup's LDS
 
-  // Lane l holds channels 4 * (l / 16) .. + 3 of row l % 16 of every 16 x 16 product.
-  const int n = n0 + wave * 16 + (lane >> 4) * 4;
-  if (n >= out_columns) return;
-  const float* b_scales = a.b_scales + static_cast<size_t>(tile.expert) * a.out_features + n;
+  // Lane l holds row l % 32 and channels 8 g + 4 (l / 32) + 0..3.
+  const int row = mw * 32 + r;
+  if (row >= tile.rows) return;
+  const float row_scale = a.a_scales[static_cast<size_t>(tile.first + row) * a.a_scales_row_stride];
 #pragma unroll
-  for (int m = 0; m < kTileM / 16; ++m) {
-    const int r = m * 16 + (lane & 15);
-    if (r >= tile.rows) continue;
-    const float row_scale = a.a_scales[static_cast<size_t>(tile.first + r) * a.a_scales_row_stride];
+  for (int g = 0; g < 4; ++g) {
+    const int n = n0 + nw * 32 + g * 8 + (lane >> 5) * 4;
+    if (n >= columns) break;
+    const float* scales = a.b_scales + static_cast<size_t>(tile.expert) * a.out_features + n;
     float o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      o[i] = static_cast<float>(acc[0][m][i]) * (row_scale * b_scales[i]);
-      if constexpr (kSilu) o[i] = silu(o[i]) * (static_cast<float>(acc[kSets - 1][m][i]) * (row_scale * b_scales[out_columns + i]));
+      o[i] = static_cast<float>(acc[0][g * 4 + i]) * (row_scale * scales[i]);
+      if constexpr (kSilu) o[i] = silu(o[i]) * (static_cast<float>(acc[kSets - 1][g * 4 + i]) * (row_scale * scales[columns + i]));
     }
-    *reinterpret_cast<uint2*>(a.out + static_cast<size_t>(tile.first + r) * out_columns + n) =
-        uint2{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
+    *reinterpret_cast<uint2*>(a.out + static_cast<size_t>(tile.first + row) * columns + n) =
+        uint2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])};
+  }
+}
+
+// ---- large tiles ------------------------------------------------------------------------------------
+constexpr int kBigM = 256, kBigN = 256;  // one stage: 64 bytes of k for 256 rows and 256 channels
+constexpr int kBigThreads = 256;
+constexpr int kStages = 4;
+constexpr int kRowGroup = 8;
+constexpr int kOperandBytes = kBigM * kBigK;                   // 16 KiB
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kRingBytes = kStages * kStageBytes;              // 128 KiB
+constexpr int kEpiloguePitch = 64 * 2 + 16;                    // 64 columns of bf16, rows shifted by four banks
+constexpr int kEpilogueBytes = 32 * kEpiloguePitch;            // one wave's 32 rows
+constexpr int kTableAt = kRingBytes + 4 * kEpilogueBytes;       // row tiles before every expert
+constexpr int kScalesAt = kTableAt + (kMaxExperts + 4) * 4;     // two tiles' 256 row and 256 channel scales
+constexpr int kBigLds = kScalesAt + 2 * 2048;
+static_assert(kBigLds <= 160 * 1024, "one workgroup takes a compute unit's LDS");
+
+struct BigTile {
+  int expert, column;  // first output column
+  int first, rows;     // rows of a
+};
+
+// One workgroup's walk over its tiles.  Wave (mw, nw) owns the 32-row blocks mw, mw + 2, ... and 128 of the 256
+// channels (with kSilu 64 gate channels and the 64 up channels of the same columns).
+template <bool kSilu>
+struct BigMatmul {
+  static constexpr int kColumns = kSilu ? kBigN / 2 : kBigN;  // output columns of a tile
+  const ExpertMatmulArgs& a;
+  unsigned char* const lds;
+  const int lds_base, lane, wave, mw, nw, K, columns, steps;
+  int4v desc_a, desc_b;
+
+  // The same value, but not the same for the compiler: what is derived from it is computed where it is used
+  // instead of being kept in registers across the tile loop, where it would be spilled.
+  static __device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  }
+  __device__ __forceinline__ BigMatmul(const ExpertMatmulArgs& args, unsigned char* shared)
+      : a(args),
+        lds(shared),
+        lds_base(lds_address(shared)),
+        lane(lane_id()),
+        wave(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6)),
+        mw(wave & 1),
+        nw(wave >> 1),
+        K(args.in_features),
+        columns(kSilu ? args.out_features / 2 : args.out_features),
+        steps((args.in_features + kBigK - 1) / kBigK) {}
+
+  // One of the wave's eight loads of a stage: 16 rows of the weights (j < 4) or of the tokens.
+  __device__ __forceinline__ void load(const Place& at, int step, int j, bool inside) const {
+    const int to = lds_base + (step & (kStages - 1)) * kStageBytes + (wave * 4 + (j & 3)) * kChunkBytes;
+    const int row = (kSilu && j < 4 ? wave & 1 : wave) * 64 + at.row + (j & 3) * 16;
+    const int offset = inside ? row * K + at.piece : kOutside;
+    if (j < 4) load_to_lds(desc_b, to + kOperandBytes, offset, step * kBigK);
+    else load_to_lds(desc_a, to, offset, step * kBigK);
+  }
+
+  // Points the descriptors at a tile and starts its scales' and first three stages' loads.
+  __device__ __forceinline__ void start(const BigTile& tile, int scales_at) {
+    const int b_rows = columns - tile.column < kColumns ? columns - tile.column : kColumns;
+    const size_t channel = static_cast<size_t>(tile.expert) * a.out_features + (kSilu && wave >= 2 ? columns : 0) + tile.column;
+    desc_a = descriptor_of(a.a + static_cast<size_t>(tile.first) * K, tile.rows * K);
+    desc_b = descriptor_of(a.b + channel * K, b_rows * K);
+    const int stride = static_cast<int>(a.a_scales_row_stride);
+    const Place at(fresh(lane));
+    const int row = fresh(static_cast<int>(threadIdx.x));
+    load_word_to_lds(descriptor_of(a.a_scales + static_cast<size_t>(tile.first) * a.a_scales_row_stride,
+                                   ((tile.rows - 1) * stride + 1) * 4),
+                     scales_at + wave * 256, row < tile.rows ? row * stride * 4 : kOutside);
+    load_word_to_lds(descriptor_of(a.b_scales + channel, b_rows * 4), scales_at + 1024 + wave * 256,
+                     (kSilu ? row & 127 : row) * 4);
+#pragma unroll
+    for (int s = 0; s < 3; ++s)
+      if (s < steps) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load(at, s, j, s * kBigK + at.piece < K);
+      }
+  }
+
+  template <int kBlocks>
+  struct Fragments {
+    int4v a[2][kBlocks], b[2][4];
+  };
+  // Fragment q of a half-step: four of channels, then the rows'.  Lane l takes row l % 32 of a block and piece
+  // 2 * half + l / 32.
+  template <int kBlocks>
+  __device__ __forceinline__ void read(const Place& at, Fragments<kBlocks>& f, int step, int half, int q) const {
+    const unsigned char* base = lds + (step & (kStages - 1)) * kStageBytes + (at.read_at ^ (half * 32));
+    if (q < 4) {
+      const int block = kSilu ? (q & 1) + nw * 2 + (q >> 1) * 4 : nw * 4 + q;
+      f.b[half][q] = *reinterpret_cast<const int4v*>(base + kOperandBytes + block * 2048);
+    } else {
+      f.a[half][q - 4] = *reinterpret_cast<const int4v*>(base + (2 * (q - 4) + mw) * 2048);
+    }
+  }
+
+  // Half a step: the products of one half's fragments; between them the reads of the next half's fragments
+  // and half of the loads of stage step + 3, one to a product.
+  template <int kBlocks, int kHalf, bool kLoad>
+  __device__ __forceinline__ void half_step(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int step) const {
+    constexpr int kLoads = kLoad ? 4 : 0;
+    constexpr int kProducts = 4 * kBlocks, kReads = 4 + kBlocks, kItems = kReads + kLoads;
+    const bool inside = (step + 3) * kBigK + at.piece < K;
+#pragma unroll
+    for (int p = 0; p < kProducts; ++p) {
+#pragma unroll
+      for (int i = p * kItems / kProducts; i < (p + 1) * kItems / kProducts; ++i) {
+        const int loads_before = kLoads == 0 ? 0 : (i + 1) * kLoads / kItems;
+        const bool is_load = kLoads != 0 && loads_before != i * kLoads / kItems;
+        if (is_load) load(at, step + 3, kHalf * 4 + loads_before - 1, inside);
+        else read<kBlocks>(at, f, kHalf == 0 ? step : step + 1, 1 - kHalf, i - loads_before);
+      }
+      acc[p / 4][p % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[kHalf][p % 4], f.a[kHalf][p / 4], acc[p / 4][p % 4], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+  // The products of one tile whose rows fill kBlocks pairs of 32-row blocks, the start of the next tile, and
+  // the epilogue.
+  template <int kBlocks>
+  __device__ __forceinline__ void run(const BigTile& tile, int scales_at, bool has_next, const BigTile& next, int next_scales_at) {
+    const Place at(fresh(lane));
+    int16v acc[kBlocks][4];
+    Fragments<kBlocks> f;
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[m][j] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+
+    if (steps > 2)
+      wait_and_meet<16 + kStores>();
+    else
+      wait_and_meet<kStores>();
+#pragma unroll
+    for (int q = 0; q < 4 + kBlocks; ++q) read<kBlocks>(at, f, 0, 0, q);
+    // The barrier in the middle of step s makes stage s + 1 visible, whose loads were issued in step s - 2 (12
+    // younger ones, and at first the previous tile's stores, may still be on their way), and tells that every
+    // wave is done with reading stage s, whose place the loads of step s + 1 fill.
+    int step = 0;
+    for (; step < 2 && step + 3 < steps; ++step) {
+      half_step<kBlocks, 0, true>(at, f, acc, step);
+      wait_and_meet<12 + kStores>();
+      half_step<kBlocks, 1, true>(at, f, acc, step);
+    }
+    for (; step + 3 < steps; ++step) {
+      half_step<kBlocks, 0, true>(at, f, acc, step);
+      wait_and_meet<12>();
+      half_step<kBlocks, 1, true>(at, f, acc, step);
+    }
+    for (; step < steps; ++step) {
+      half_step<kBlocks, 0, false>(at, f, acc, step);
+      wait_and_meet<0>();
+      half_step<kBlocks, 1, false>(at, f, acc, step);
+    }
+    // The next tile's loads run during this one's epilogue.
+    if (has_next) start(next, next_scales_at);
+
+    // Lane l holds row l % 32 of a block and channels 8 g + 4 (l / 32) + 0..3; through the wave's own piece of
+    // LDS they become rows of 64 columns, stored 16 bytes a lane.
+    const int lane = fresh(this->lane), r = lane & 31;
+    unsigned char* mine = lds + kRingBytes + wave * kEpilogueBytes;
+    const float* row_scales = reinterpret_cast<const float*>(lds + (scales_at - lds_base));
+    const float* b_scales = row_scales + 256;
+    const int wave_column = nw * (kSilu ? 64 : 128);  // in the tile
+    const __amdgpu_buffer_rsrc_t out = out_rows(tile);
+#pragma unroll
+    for (int m = 0; m < kBlocks; ++m) {
+      const int row0 = (2 * m + mw) * 32;
+      const float row_scale = row_scales[row0 + r];
+#pragma unroll
+      for (int part = 0; part < (kSilu ? 1 : 2); ++part) {
+        const int column0 = wave_column + part * 64;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int j = part * 2 + jj;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int c = jj * 32 + g * 8 + (lane >> 5) * 4;
+            const float4 s4 = *reinterpret_cast<const float4*>(b_scales + column0 + c);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+            float o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(acc[m][j][g * 4 + i]) * (row_scale * s[i]);
+            if constexpr (kSilu) {
+              const float4 t4 = *reinterpret_cast<const float4*>(b_scales + 128 + column0 + c);
+              const float u[4] = {t4.x, t4.y, t4.z, t4.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + 2) & 3][g * 4 + i]) * (row_scale * u[i]));
+            }
+            *reinterpret_cast<uint2*>(mine + r * kEpiloguePitch + c * 2) = uint2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])};
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int local = q * 8 + (lane >> 3), c = (lane & 7) * 8;
+          const vec16 v = *reinterpret_cast<const vec16*>(mine + local * kEpiloguePitch + c * 2);
+          const int column = tile.column + column0 + c;
+          __builtin_amdgcn_raw_buffer_store_b128(v, out, column < columns ? ((row0 + local) * columns + column) * 2 : kOutside, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one part's values at a time: more would not fit the registers
+      }
+    }
+    idle_stores<(4 - kBlocks) * kStores / 4>(out);
+  }
+
+  // The waits of the next tile's first steps count the stores of this one, so every tile issues as many: rows
+  // behind the tile's and columns behind the matrix lie outside the descriptor and go nowhere.
+  static constexpr int kStores = kSilu ? 16 : 32;
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t out_rows(const BigTile& tile) const {
+    return __builtin_amdgcn_make_buffer_rsrc(a.out + static_cast<size_t>(tile.first) * columns, 0, tile.rows * columns * 2,
+                                             kRawBufferFormat);
+  }
+  template <int kCount>
+  __device__ __forceinline__ void idle_stores(__amdgpu_buffer_rsrc_t out) const {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) __builtin_amdgcn_raw_buffer_store_b128(vec16{0, 0, 0, 0}, out, kOutside, i, 0);
+  }
+  // Until at most kYounger of the wave's memory operations are on their way and its LDS reads are back, then
+  // until every wave got there.
+  template <int kYounger>
+  static __device__ __forceinline__ void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kYounger) : "memory");
+  }
+};
+
+template <bool kSilu>
+__global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(const ExpertMatmulArgs a) {
+  extern __shared__ __align__(1024) unsigned char lds[];
+  int* tiles_before = reinterpret_cast<int*>(lds + kTableAt);  // [num_experts + 1]
+  const int t = static_cast<int>(threadIdx.x);
+  {  // row tiles before every expert: up to four experts a thread, scanned over the workgroup
+    int* wave_total = reinterpret_cast<int*>(lds);
+    const int per = (a.num_experts + kBigThreads - 1) / kBigThreads;
+    int count[kMaxExperts / kBigThreads], mine = 0;
+#pragma unroll
+    for (int j = 0; j < kMaxExperts / kBigThreads; ++j) {
+      const int e = t * per + j;
+      count[j] = j < per && e < a.num_experts ? (segment_of(a, e).rows + kBigM - 1) / kBigM : 0;
+      mine += count[j];
+    }
+    const int upto = wave_inclusive_scan(mine);
+    if (lane_id() == kWave - 1) wave_total[t >> 6] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    for (int w = 0; w < (t >> 6); ++w) before += wave_total[w];
+#pragma unroll
+    for (int j = 0; j < kMaxExperts / kBigThreads; ++j) {
+      const int e = t * per + j;
+      if (j < per && e < a.num_experts) tiles_before[e] = before;
+      before += count[j];
+    }
+    if (t == kBigThreads - 1) tiles_before[a.num_experts] = before;
+    __syncthreads();
+  }
+  BigMatmul<kSilu> matmul(a, lds);
+  constexpr int kColumns = BigMatmul<kSilu>::kColumns;
+  const int column_tiles = (matmul.columns + kColumns - 1) / kColumns;
+  const auto locate = [&](int index) {
+    const int row_tile_times = index / column_tiles;
+    int lo = 0, hi = a.num_experts;  // tiles_before[lo] <= row_tile_times < tiles_before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__builtin_amdgcn_readfirstlane(tiles_before[mid]) <= row_tile_times) lo = mid;
+      else hi = mid;
+    }
+    const int first_tile = __builtin_amdgcn_readfirstlane(tiles_before[lo]);
+    const int row_tiles = __builtin_amdgcn_readfirstlane(tiles_before[lo + 1]) - first_tile;
+    // Inside an expert: groups of up to eight row tiles by as many columns as make about 32 tiles, one die's share
+    // at a time, so that rows and weights are each fetched once for all of them; columns fastest, so that a
+    // group's short last row of tiles is shared out over all compute units and not always to the same ones.
+    const int inside = index - first_tile * column_tiles;
+    const int group = inside / (kRowGroup * column_tiles);
+    const int in_group = inside - group * kRowGroup * column_tiles;
+    const int rows_left = row_tiles - group * kRowGroup;
+    const int group_rows = rows_left < kRowGroup ? rows_left : kRowGroup;
+    const int chunk_columns = 32 / group_rows;
+    const int chunk = in_group / (group_rows * chunk_columns);
+    const int in_chunk = in_group - chunk * group_rows * chunk_columns;
+    const int columns_left = column_tiles - chunk * chunk_columns;
+    const int width = columns_left < chunk_columns ? columns_left : chunk_columns;
+    const int row_in_group = in_chunk / width;
+    const int row_tile = group * kRowGroup + row_in_group, column_tile = chunk * chunk_columns + in_chunk - row_in_group * width;
+    const Segment all = segment_of(a, lo);
+    const int left = __builtin_amdgcn_readfirstlane(all.rows) - row_tile * kBigM;
+    return BigTile{lo, column_tile * kColumns, __builtin_amdgcn_readfirstlane(all.first) + row_tile * kBigM,
+                   left < kBigM ? left : kBigM};
+  };
+
+  // Workgroups go to the eight dies in turn; each die takes one contiguous run of the tiles, so that the rows
+  // and weights its compute units share come from its own L2.
+  const int total = __builtin_amdgcn_readfirstlane(tiles_before[a.num_experts]) * column_tiles;
+  const int dies = gridDim.x % 8 == 0 ? 8 : 1;
+  const int per_die = (total + dies - 1) / dies;
+  const int die = static_cast<int>(blockIdx.x) % dies;
+  const int end = (die + 1) * per_die < total ? (die + 1) * per_die : total;
+  const int stride = static_cast<int>(gridDim.x) / dies;
+  int index = die * per_die + static_cast<int>(blockIdx.x) / dies;
+  if (index >= end) return;
+  const int scales_at = matmul.lds_base + kScalesAt;
+  int turn = 0;
+  BigTile tile = locate(index);
+  matmul.start(tile, scales_at);
+  matmul.template idle_stores<BigMatmul<kSilu>::kStores>(matmul.out_rows(tile));
+  for (;;) {
+    index += stride;
+    const bool has_next = index < end;
+    const BigTile next = has_next ? locate(index) : tile;
+    const int at = scales_at + turn * 2048, next_at = scales_at + (turn ^ 1) * 2048;
+    switch ((tile.rows + 63) / 64) {
+      case 1: matmul.template run<1>(tile, at, has_next, next, next_at); break;
+      case 2: matmul.template run<2>(tile, at, has_next, next, next_at); break;
+      case 3: matmul.template run<3>(tile, at, has_next, next, next_at); break;
+      default: matmul.template run<4>(tile, at, has_next, next, next_at); break;
+    }
+    if (!has_next) return;
+    tile = next;
+    turn ^= 1;
   }
 }
 
@@ -140,14 +543,26 @@ __global__ __launch_bounds__(256) void ep_expert_matmul_kernel(const ExpertMatmu
 hipError_t launch_expert_matmul(const ExpertMatmulArgs& a, hipStream_t stream) {
   if (a.num_rows == 0) return hipSuccess;
   const int columns = a.silu_mul ? a.out_features / 2 : a.out_features;
+  static const char* big = getenv("EPBIG");
+  if (big != nullptr ? big[0] == '1' : true) {
+    const void* kernel = a.silu_mul ? reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<true>)
+                                    : reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<false>);
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds);
+    if (e != hipSuccess) return e;
+    if (a.silu_mul)
+      hipLaunchKernelGGL((ep_expert_matmul_big_kernel<true>), dim3(256), dim3(kBigThreads), kBigLds, stream, a);
+    else
+      hipLaunchKernelGGL((ep_expert_matmul_big_kernel<false>), dim3(256), dim3(kBigThreads), kBigLds, stream, a);
+    return hipGetLastError();
+  }
   // Every segment ends in at most one partial tile.
   const int row_tiles = a.num_rows / kTileM + a.num_experts;
   if (row_tiles > 65535) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>((columns + kTileN - 1) / kTileN), static_cast<unsigned>(row_tiles));
   if (a.silu_mul)
-    hipLaunchKernelGGL((ep_expert_matmul_kernel<true>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((ep_expert_matmul_small_kernel<true>), grid, dim3(kSmallThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((ep_expert_matmul_kernel<false>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((ep_expert_matmul_small_kernel<false>), grid, dim3(kSmallThreads), 0, stream, a);
   return hipGetLastError();
 }
 
