@@ -3,7 +3,7 @@
 //   c[m, n] = a_scale[m] * b_scale[e, n] * sum_k a[m, k] * b[e, n, k]     rows m of expert e's segment
 //   out = bf16(c)   or, gate and up in one product,   out[m, i] = bf16(silu(c[m, i]) * c[m, I + i])
 // The sum over k is exact in 32-bit integers (|a|, |b| <= 128 and k < 2^17).
-#include <cstdlib>
+#include <atomic>
 #include "ep_device.h"
 
 namespace mi_ep {
@@ -218,19 +218,27 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
 }
 
 // ---- large tiles ------------------------------------------------------------------------------------
-constexpr int kBigM = 256, kBigN = 256;  // one stage: 64 bytes of k for 256 rows and 256 channels
+constexpr int kBigN = 256;       // channels of a tile: with kSilu 128 gate channels and their 128 up channels
+constexpr int kBlockRows = 64;   // a tile's rows come in pairs of 32-row blocks, one for each half of the waves
+constexpr int kMaxBlocks = 4;    // 256 rows: the accumulators fill the matrix units' own registers
 constexpr int kBigThreads = 256;
 constexpr int kStages = 4;
 constexpr int kRowGroup = 8;
-constexpr int kOperandBytes = kBigM * kBigK;                   // 16 KiB
-constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kRingBytes = kStages * kStageBytes;              // 128 KiB
-constexpr int kEpiloguePitch = 64 * 2 + 16;                    // 64 columns of bf16, rows shifted by four banks
-constexpr int kEpilogueBytes = 32 * kEpiloguePitch;            // one wave's 32 rows
-constexpr int kTableAt = kRingBytes + 4 * kEpilogueBytes;       // row tiles before every expert
-constexpr int kScalesAt = kTableAt + (kMaxExperts + 4) * 4;     // two tiles' 256 row and 256 channel scales
-constexpr int kBigLds = kScalesAt + 2 * 2048;
+constexpr int kABytes = kMaxBlocks * kBlockRows * kBigK;     // 16 KiB: a stage is 64 bytes of k of the rows
+constexpr int kStageBytes = kABytes + kBigN * kBigK;         // and 16 KiB of the channels
+constexpr int kRingBytes = kStages * kStageBytes;            // 128 KiB
+constexpr int kEpiloguePitch = 64 * 2 + 16;                  // 64 columns of bf16, rows shifted by four banks
+constexpr int kEpilogueBytes = 32 * kEpiloguePitch;          // one wave's 32 rows
+constexpr int kTableAt = kRingBytes + 4 * kEpilogueBytes;    // row tiles before every thread's experts
+constexpr int kRowScaleBytes = kMaxBlocks * kBlockRows * 4;
+constexpr int kScaleBytes = kRowScaleBytes + kBigN * 4;
+constexpr int kScalesAt = kTableAt + (kBigThreads + 4) * 4;  // two tiles' row and channel scales
+constexpr int kBigLds = kScalesAt + 2 * kScaleBytes;
 static_assert(kBigLds <= 160 * 1024, "one workgroup takes a compute unit's LDS");
+
+// Row tiles of a segment of so many pairs of blocks: as few as possible, each with blocks / tiles of them, rounded
+// down or up.
+__device__ __forceinline__ int row_tiles_of(int blocks) { return (blocks + kMaxBlocks - 1) / kMaxBlocks; }
 
 struct BigTile {
   int expert, column;  // first output column
@@ -265,13 +273,16 @@ struct BigMatmul {
         columns(kSilu ? args.out_features / 2 : args.out_features),
         steps((args.in_features + kBigK - 1) / kBigK) {}
 
-  // One of the wave's eight loads of a stage: 16 rows of the weights (j < 4) or of the tokens.
-  __device__ __forceinline__ void load(const Place& at, int step, int j, bool inside) const {
-    const int to = lds_base + (step & (kStages - 1)) * kStageBytes + (wave * 4 + (j & 3)) * kChunkBytes;
-    const int row = (kSilu && j < 4 ? wave & 1 : wave) * 64 + at.row + (j & 3) * 16;
-    const int offset = inside ? row * K + at.piece : kOutside;
-    if (j < 4) load_to_lds(desc_b, to + kOperandBytes, offset, step * kBigK);
-    else load_to_lds(desc_a, to, offset, step * kBigK);
+  // Load j of a stage: 16 rows of the channels, or 16 rows of the tokens.
+  __device__ __forceinline__ void load_b(const Place& at, int step, int j, bool inside) const {
+    const int to = lds_base + (step & (kStages - 1)) * kStageBytes + kABytes + (wave * 4 + j) * kChunkBytes;
+    const int row = (kSilu ? wave & 1 : wave) * 64 + at.row + j * 16;
+    load_to_lds(desc_b, to, inside ? row * K + at.piece : kOutside, step * kBigK);
+  }
+  __device__ __forceinline__ void load_a(const Place& at, int step, int j, bool inside) const {
+    const int to = lds_base + (step & (kStages - 1)) * kStageBytes + (j * 4 + wave) * kChunkBytes;
+    const int row = (j * 4 + wave) * 16 + at.row;
+    load_to_lds(desc_a, to, inside ? row * K + at.piece : kOutside, step * kBigK);
   }
 
   // Points the descriptors at a tile and starts its scales' and first three stages' loads.
@@ -283,17 +294,20 @@ struct BigMatmul {
     const int stride = static_cast<int>(a.a_scales_row_stride);
     const Place at(fresh(lane));
     const int row = fresh(static_cast<int>(threadIdx.x));
-    load_word_to_lds(descriptor_of(a.a_scales + static_cast<size_t>(tile.first) * a.a_scales_row_stride,
-                                   ((tile.rows - 1) * stride + 1) * 4),
-                     scales_at + wave * 256, row < tile.rows ? row * stride * 4 : kOutside);
-    load_word_to_lds(descriptor_of(a.b_scales + channel, b_rows * 4), scales_at + 1024 + wave * 256,
+    const int4v desc_scales = descriptor_of(a.a_scales + static_cast<size_t>(tile.first) * a.a_scales_row_stride,
+                                            ((tile.rows - 1) * stride + 1) * 4);
+    load_word_to_lds(desc_scales, scales_at + wave * 256, row < tile.rows ? row * stride * 4 : kOutside);
+    load_word_to_lds(descriptor_of(a.b_scales + channel, b_rows * 4), scales_at + kRowScaleBytes + wave * 256,
                      (kSilu ? row & 127 : row) * 4);
+    const int blocks = (tile.rows + kBlockRows - 1) / kBlockRows;
+    for (int s = 0; s < 3 && s < steps; ++s) {
+      const bool inside = s * kBigK + at.piece < K;
 #pragma unroll
-    for (int s = 0; s < 3; ++s)
-      if (s < steps) {
+      for (int j = 0; j < 4; ++j) load_b(at, s, j, inside);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) load(at, s, j, s * kBigK + at.piece < K);
-      }
+      for (int j = 0; j < kMaxBlocks; ++j)
+        if (j < blocks) load_a(at, s, j, inside);
+    }
   }
 
   template <int kBlocks>
@@ -307,17 +321,17 @@ struct BigMatmul {
     const unsigned char* base = lds + (step & (kStages - 1)) * kStageBytes + (at.read_at ^ (half * 32));
     if (q < 4) {
       const int block = kSilu ? (q & 1) + nw * 2 + (q >> 1) * 4 : nw * 4 + q;
-      f.b[half][q] = *reinterpret_cast<const int4v*>(base + kOperandBytes + block * 2048);
+      f.b[half][q] = *reinterpret_cast<const int4v*>(base + kABytes + block * 2048);
     } else {
       f.a[half][q - 4] = *reinterpret_cast<const int4v*>(base + (2 * (q - 4) + mw) * 2048);
     }
   }
 
   // Half a step: the products of one half's fragments; between them the reads of the next half's fragments
-  // and half of the loads of stage step + 3, one to a product.
+  // and the loads of stage step + 3, of the channels in the first half and of the rows in the second.
   template <int kBlocks, int kHalf, bool kLoad>
   __device__ __forceinline__ void half_step(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int step) const {
-    constexpr int kLoads = kLoad ? 4 : 0;
+    constexpr int kLoads = !kLoad ? 0 : kHalf == 0 ? 4 : kBlocks;
     constexpr int kProducts = 4 * kBlocks, kReads = 4 + kBlocks, kItems = kReads + kLoads;
     const bool inside = (step + 3) * kBigK + at.piece < K;
 #pragma unroll
@@ -326,7 +340,7 @@ struct BigMatmul {
       for (int i = p * kItems / kProducts; i < (p + 1) * kItems / kProducts; ++i) {
         const int loads_before = kLoads == 0 ? 0 : (i + 1) * kLoads / kItems;
         const bool is_load = kLoads != 0 && loads_before != i * kLoads / kItems;
-        if (is_load) load(at, step + 3, kHalf * 4 + loads_before - 1, inside);
+        if (is_load) kHalf == 0 ? load_b(at, step + 3, loads_before - 1, inside) : load_a(at, step + 3, loads_before - 1, inside);
         else read<kBlocks>(at, f, kHalf == 0 ? step : step + 1, 1 - kHalf, i - loads_before);
       }
       acc[p / 4][p % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[kHalf][p % 4], f.a[kHalf][p / 4], acc[p / 4][p % 4], 0, 0, 0);
@@ -346,24 +360,25 @@ struct BigMatmul {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[m][j] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
+    constexpr int kStageLoads = 4 + kBlocks;
     if (steps > 2)
-      wait_and_meet<16 + kStores>();
+      wait_and_meet<2 * kStageLoads + kStores>();
     else
       wait_and_meet<kStores>();
 #pragma unroll
     for (int q = 0; q < 4 + kBlocks; ++q) read<kBlocks>(at, f, 0, 0, q);
-    // The barrier in the middle of step s makes stage s + 1 visible, whose loads were issued in step s - 2 (12
-    // younger ones, and at first the previous tile's stores, may still be on their way), and tells that every
-    // wave is done with reading stage s, whose place the loads of step s + 1 fill.
+    // The barrier in the middle of step s makes stage s + 1 visible, whose loads were issued in step s - 2 (those
+    // of step s - 1, four of step s and at first the previous tile's stores may still be on their way), and
+    // tells that every wave is done with reading stage s, whose place the loads of step s + 1 fill.
     int step = 0;
     for (; step < 2 && step + 3 < steps; ++step) {
       half_step<kBlocks, 0, true>(at, f, acc, step);
-      wait_and_meet<12 + kStores>();
+      wait_and_meet<kStageLoads + 4 + kStores>();
       half_step<kBlocks, 1, true>(at, f, acc, step);
     }
     for (; step + 3 < steps; ++step) {
       half_step<kBlocks, 0, true>(at, f, acc, step);
-      wait_and_meet<12>();
+      wait_and_meet<kStageLoads + 4>();
       half_step<kBlocks, 1, true>(at, f, acc, step);
     }
     for (; step < steps; ++step) {
@@ -379,8 +394,7 @@ struct BigMatmul {
     const int lane = fresh(this->lane), r = lane & 31;
     unsigned char* mine = lds + kRingBytes + wave * kEpilogueBytes;
     const float* row_scales = reinterpret_cast<const float*>(lds + (scales_at - lds_base));
-    const float* b_scales = row_scales + 256;
-    const int wave_column = nw * (kSilu ? 64 : 128);  // in the tile
+    const float* b_scales = row_scales + kRowScaleBytes / 4;
     const __amdgpu_buffer_rsrc_t out = out_rows(tile);
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) {
@@ -388,7 +402,7 @@ struct BigMatmul {
       const float row_scale = row_scales[row0 + r];
 #pragma unroll
       for (int part = 0; part < (kSilu ? 1 : 2); ++part) {
-        const int column0 = wave_column + part * 64;
+        const int column0 = nw * (kSilu ? 64 : 128) + part * 64;  // in the tile
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj) {
           const int j = part * 2 + jj;
@@ -420,12 +434,12 @@ struct BigMatmul {
         __builtin_amdgcn_sched_barrier(0);  // one part's values at a time: more would not fit the registers
       }
     }
-    idle_stores<(4 - kBlocks) * kStores / 4>(out);
+    idle_stores<(kMaxBlocks - kBlocks) * kStores / kMaxBlocks>(out);
   }
 
   // The waits of the next tile's first steps count the stores of this one, so every tile issues as many: rows
   // behind the tile's and columns behind the matrix lie outside the descriptor and go nowhere.
-  static constexpr int kStores = kSilu ? 16 : 32;
+  static constexpr int kStores = kMaxBlocks * (kSilu ? 4 : 8);
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t out_rows(const BigTile& tile) const {
     return __builtin_amdgcn_make_buffer_rsrc(a.out + static_cast<size_t>(tile.first) * columns, 0, tile.rows * columns * 2,
                                              kRawBufferFormat);
@@ -446,30 +460,25 @@ struct BigMatmul {
 template <bool kSilu>
 __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(const ExpertMatmulArgs a) {
   extern __shared__ __align__(1024) unsigned char lds[];
-  int* tiles_before = reinterpret_cast<int*>(lds + kTableAt);  // [num_experts + 1]
+  constexpr int kPer = kMaxExperts / kBigThreads;
+  int* tiles_before = reinterpret_cast<int*>(lds + kTableAt);  // [kBigThreads + 1], before the experts of every thread
   const int t = static_cast<int>(threadIdx.x);
-  {  // row tiles before every expert: up to four experts a thread, scanned over the workgroup
+  const int per = (a.num_experts + kBigThreads - 1) / kBigThreads;
+  const auto tiles_of = [&](int e) {
+    return e < a.num_experts ? row_tiles_of((segment_of(a, e).rows + kBlockRows - 1) / kBlockRows) : 0;
+  };
+  {
     int* wave_total = reinterpret_cast<int*>(lds);
-    const int per = (a.num_experts + kBigThreads - 1) / kBigThreads;
-    int count[kMaxExperts / kBigThreads], mine = 0;
+    int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kMaxExperts / kBigThreads; ++j) {
-      const int e = t * per + j;
-      count[j] = j < per && e < a.num_experts ? (segment_of(a, e).rows + kBigM - 1) / kBigM : 0;
-      mine += count[j];
-    }
+    for (int j = 0; j < kPer; ++j) mine += j < per ? tiles_of(t * per + j) : 0;
     const int upto = wave_inclusive_scan(mine);
     if (lane_id() == kWave - 1) wave_total[t >> 6] = upto;
     __syncthreads();
     int before = upto - mine;
     for (int w = 0; w < (t >> 6); ++w) before += wave_total[w];
-#pragma unroll
-    for (int j = 0; j < kMaxExperts / kBigThreads; ++j) {
-      const int e = t * per + j;
-      if (j < per && e < a.num_experts) tiles_before[e] = before;
-      before += count[j];
-    }
-    if (t == kBigThreads - 1) tiles_before[a.num_experts] = before;
+    tiles_before[t] = before;
+    if (t == kBigThreads - 1) tiles_before[kBigThreads] = before + mine;
     __syncthreads();
   }
   BigMatmul<kSilu> matmul(a, lds);
@@ -477,17 +486,26 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
   const int column_tiles = (matmul.columns + kColumns - 1) / kColumns;
   const auto locate = [&](int index) {
     const int row_tile_times = index / column_tiles;
-    int lo = 0, hi = a.num_experts;  // tiles_before[lo] <= row_tile_times < tiles_before[hi]
+    int lo = 0, hi = kBigThreads;  // tiles_before[lo] <= row_tile_times < tiles_before[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (__builtin_amdgcn_readfirstlane(tiles_before[mid]) <= row_tile_times) lo = mid;
       else hi = mid;
     }
-    const int first_tile = __builtin_amdgcn_readfirstlane(tiles_before[lo]);
-    const int row_tiles = __builtin_amdgcn_readfirstlane(tiles_before[lo + 1]) - first_tile;
+    int first_tile = __builtin_amdgcn_readfirstlane(tiles_before[lo]);
+    int expert = lo * per;
+    for (int j = 1; j < per; ++j) {  // up to three more experts of the same thread
+      const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(expert));
+      if (first_tile + tiles > row_tile_times) break;
+      first_tile += tiles;
+      ++expert;
+    }
+    const Segment all = segment_of(a, expert);
+    const int rows = __builtin_amdgcn_readfirstlane(all.rows);
+    const int blocks = (rows + kBlockRows - 1) / kBlockRows, row_tiles = row_tiles_of(blocks);
     // Inside an expert: groups of up to eight row tiles by as many columns as make about 32 tiles, one die's share
     // at a time, so that rows and weights are each fetched once for all of them; columns fastest, so that a
-    // group's short last row of tiles is shared out over all compute units and not always to the same ones.
+    // group's shorter tiles are shared out over all compute units and not always to the same ones.
     const int inside = index - first_tile * column_tiles;
     const int group = inside / (kRowGroup * column_tiles);
     const int in_group = inside - group * kRowGroup * column_tiles;
@@ -500,15 +518,15 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
     const int width = columns_left < chunk_columns ? columns_left : chunk_columns;
     const int row_in_group = in_chunk / width;
     const int row_tile = group * kRowGroup + row_in_group, column_tile = chunk * chunk_columns + in_chunk - row_in_group * width;
-    const Segment all = segment_of(a, lo);
-    const int left = __builtin_amdgcn_readfirstlane(all.rows) - row_tile * kBigM;
-    return BigTile{lo, column_tile * kColumns, __builtin_amdgcn_readfirstlane(all.first) + row_tile * kBigM,
-                   left < kBigM ? left : kBigM};
+    const int from = static_cast<int>(static_cast<long long>(row_tile) * blocks / row_tiles) * kBlockRows;
+    const int to = static_cast<int>(static_cast<long long>(row_tile + 1) * blocks / row_tiles) * kBlockRows;
+    return BigTile{expert, column_tile * kColumns, __builtin_amdgcn_readfirstlane(all.first) + from,
+                   (to < rows ? to : rows) - from};
   };
 
   // Workgroups go to the eight dies in turn; each die takes one contiguous run of the tiles, so that the rows
   // and weights its compute units share come from its own L2.
-  const int total = __builtin_amdgcn_readfirstlane(tiles_before[a.num_experts]) * column_tiles;
+  const int total = __builtin_amdgcn_readfirstlane(tiles_before[kBigThreads]) * column_tiles;
   const int dies = gridDim.x % 8 == 0 ? 8 : 1;
   const int per_die = (total + dies - 1) / dies;
   const int die = static_cast<int>(blockIdx.x) % dies;
@@ -525,8 +543,8 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
     index += stride;
     const bool has_next = index < end;
     const BigTile next = has_next ? locate(index) : tile;
-    const int at = scales_at + turn * 2048, next_at = scales_at + (turn ^ 1) * 2048;
-    switch ((tile.rows + 63) / 64) {
+    const int at = scales_at + turn * kScaleBytes, next_at = scales_at + (turn ^ 1) * kScaleBytes;
+    switch ((tile.rows + kBlockRows - 1) / kBlockRows) {
       case 1: matmul.template run<1>(tile, at, has_next, next, next_at); break;
       case 2: matmul.template run<2>(tile, at, has_next, next, next_at); break;
       case 3: matmul.template run<3>(tile, at, has_next, next, next_at); break;
@@ -543,26 +561,49 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
 hipError_t launch_expert_matmul(const ExpertMatmulArgs& a, hipStream_t stream) {
   if (a.num_rows == 0) return hipSuccess;
   const int columns = a.silu_mul ? a.out_features / 2 : a.out_features;
-  static const char* big = getenv("EPBIG");
-  if (big != nullptr ? big[0] == '1' : true) {
-    const void* kernel = a.silu_mul ? reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<true>)
-                                    : reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<false>);
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds);
-    if (e != hipSuccess) return e;
+  // Large tiles where there are enough of them for most compute units and enough rows in each to be worth the
+  // accumulators.  Small / large in us: 256 experts x 4096 x 7168 with 2, 8, 16, 64 rows each: 1276 / 1314, 1307 / 1325,
+  // 1354 / 1341, 1565 / 1459; 64 large tiles (8 x 256 rows x 2048 channels, k 2048): 22 / 31, 128 of them (8 x 256 x
+  // 4096): 55 / 41, 104 (8 x 384 x 2048, k 4096): 73 / 58.
+  const long long big_columns = a.silu_mul ? kBigN / 2 : kBigN;
+  const long long by_rows = a.num_rows / (kMaxBlocks * kBlockRows);
+  const long long by_experts = a.num_rows / 12 < a.num_experts ? a.num_rows / 12 : a.num_experts;
+  const long long big_tiles = (by_rows > by_experts ? by_rows : by_experts) * ((columns + big_columns - 1) / big_columns);
+  const bool big = a.num_rows > 12LL * a.num_experts && big_tiles >= 96;
+  if (big) {
+    DeviceTraits dev{};
+    int ordinal = 0;
+    hipError_t err = device_traits(stream, &dev);
+    if (err == hipSuccess) err = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
+    if (err != hipSuccess) return err;
+    // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
+    constexpr int kMaxDevices = 64;
+    static std::atomic<int> lds_limit_raised[2][kMaxDevices];
+    if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
+    std::atomic<int>& raised = lds_limit_raised[a.silu_mul ? 1 : 0][ordinal];
+    if (raised.load(std::memory_order_acquire) == 0) {
+      const void* kernel = a.silu_mul ? reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<true>)
+                                      : reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<false>);
+      err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds);
+      if (err != hipSuccess) return err;
+      raised.store(1, std::memory_order_release);
+    }
+    const dim3 grid(static_cast<unsigned>(dev.compute_units));
     if (a.silu_mul)
-      hipLaunchKernelGGL((ep_expert_matmul_big_kernel<true>), dim3(256), dim3(kBigThreads), kBigLds, stream, a);
+      hipLaunchKernelGGL((ep_expert_matmul_big_kernel<true>), grid, dim3(kBigThreads), kBigLds, stream, a);
     else
-      hipLaunchKernelGGL((ep_expert_matmul_big_kernel<false>), dim3(256), dim3(kBigThreads), kBigLds, stream, a);
+      hipLaunchKernelGGL((ep_expert_matmul_big_kernel<false>), grid, dim3(kBigThreads), kBigLds, stream, a);
     return hipGetLastError();
   }
   // Every segment ends in at most one partial tile.
   const int row_tiles = a.num_rows / kTileM + a.num_experts;
-  if (row_tiles > 65535) return hipErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>((columns + kTileN - 1) / kTileN), static_cast<unsigned>(row_tiles));
+  const unsigned column_tiles = static_cast<unsigned>((columns + kTileN - 1) / kTileN);
   if (a.silu_mul)
-    hipLaunchKernelGGL((ep_expert_matmul_small_kernel<true>), grid, dim3(kSmallThreads), 0, stream, a);
+    hipLaunchKernelGGL((ep_expert_matmul_small_kernel<true>), dim3(column_tiles, static_cast<unsigned>(row_tiles)),
+                       dim3(kSmallThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((ep_expert_matmul_small_kernel<false>), grid, dim3(kSmallThreads), 0, stream, a);
+    hipLaunchKernelGGL((ep_expert_matmul_small_kernel<false>), dim3(column_tiles, static_cast<unsigned>(row_tiles)),
+                       dim3(kSmallThreads), 0, stream, a);
   return hipGetLastError();
 }
 
