@@ -696,7 +696,7 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
 size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int intermediate) {
   if (!few_tokens_shape_ok(num_tokens, num_topk) || intermediate <= 0 || intermediate % 16 != 0 || intermediate > 65536)
     return 0;
-  return static_cast<size_t>(num_tokens) * num_topk * (static_cast<size_t>(intermediate) * 2 + sizeof(int));
+  return static_cast<size_t>(num_tokens) * num_topk * intermediate * 2;
 }
 
 int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* topk_weights, const void* w13,
@@ -726,7 +726,6 @@ int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* to
   a.bias_0 = static_cast<const uint16_t*>(bias_0);
   a.bias_1 = static_cast<const uint16_t*>(bias_1);
   a.act = static_cast<uint16_t*>(workspace);
-  a.leaders = reinterpret_cast<int*>(a.act + static_cast<size_t>(num_tokens) * num_topk * intermediate);
   a.combined_x = static_cast<uint16_t*>(combined_x);
   a.num_tokens = num_tokens;
   a.num_topk = num_topk;

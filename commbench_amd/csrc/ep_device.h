@@ -264,7 +264,6 @@ struct FewTokensArgs {
   const uint16_t* bias_0;
   const uint16_t* bias_1;
   uint16_t* act;  // bf16 [num_tokens * num_topk, intermediate]
-  int* leaders;   // [num_tokens * num_topk]: 1 for the first route of every met expert
   uint16_t* combined_x;
   int num_tokens;
   int num_topk;

@@ -47,276 +47,385 @@ __device__ __forceinline__ bf16x8 as_bf16(vec16 v) {
   return out.b;
 }
 
-// A chunk is what 64 lanes take of 16 weight rows in one 16-byte load each: lane l has row l % 16 and the l / 16-th
-// piece of 64 contiguous bytes.  The columns' vectors are read in the same order over k, which is all a
+// A chunk is 128 contiguous bytes of 16 weight rows, whole cache lines, in two 16-byte loads of a lane: lane l has
+// row l % 16 and the l / 16-th 32 bytes.  The columns' vectors are read in the same order over k, which is all a
 // product needs.
 template <bool kInt8>
 struct Chunk {
   static constexpr int kBytes = kInt8 ? 1 : 2;
-  static constexpr int kLane = 16 / kBytes;      // elements of a lane
-  static constexpr int kElements = 4 * kLane;    // of k
-  static constexpr int kVectors = kInt8 ? 2 : 1; // 16-byte bf16 loads of a column for them
+  static constexpr int kPiece = 16 / kBytes;      // elements of a load of weights
+  static constexpr int kLane = 2 * kPiece;        // of a lane
+  static constexpr int kElements = 4 * kLane;     // of k
+  static constexpr int kVectors = kInt8 ? 2 : 1;  // 16-byte bf16 loads of a column for a load of weights
 };
-
-// acc[m][c] += W[m][16 rows] . X[16 columns of c] over chunks [begin, end) of k: kBatch chunks of weights and
-// columns are loaded before the first product, so that many bytes are on their way whatever the latency.  w_at, x_at:
-// the lane's byte offsets at k = 0; a lane without a column has kOutside.
-template <bool kInt8, int kMatrices, int kColumns, int kBatch>
-__device__ __forceinline__ void multiply(const __amdgpu_buffer_rsrc_t (&w)[kMatrices], int w_at, __amdgpu_buffer_rsrc_t x,
-                                         const int (&x_at)[kColumns], int begin, int end, int length,
-                                         float4v (&acc)[kMatrices][kColumns]) {
-  using C = Chunk<kInt8>;
-  const int k_lane = (lane_id() >> 4) * C::kLane;
-  for (int chunk = begin; chunk < end; chunk += kBatch) {
-    vec16 wv[kBatch][kMatrices], xv[kBatch][kColumns][C::kVectors];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      // Chunks behind the range, and the lanes of the last one behind the row, read nothing.
-      const bool inside = chunk + b < end && (chunk + b) * C::kElements + k_lane < length;
-      const int at = inside ? w_at + (chunk + b) * 64 : kOutside;
-#pragma unroll
-      for (int m = 0; m < kMatrices; ++m) wv[b][m] = __builtin_amdgcn_raw_buffer_load_b128(w[m], at, 0, kCachePolicyStreaming);
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c) {
-        const int from = inside ? x_at[c] + (chunk + b) * C::kElements * 2 : kOutside;
-#pragma unroll
-        for (int v = 0; v < C::kVectors; ++v) xv[b][c][v] = __builtin_amdgcn_raw_buffer_load_b128(x, from + 16 * v, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-      for (int m = 0; m < kMatrices; ++m) {
-        if constexpr (kInt8) {
-          const bf16x8 w0 = widen(wv[b][m][0], wv[b][m][1]), w1 = widen(wv[b][m][2], wv[b][m][3]);
-#pragma unroll
-          for (int c = 0; c < kColumns; ++c) {
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, as_bf16(xv[b][c][0]), acc[m][c], 0, 0, 0);
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, as_bf16(xv[b][c][C::kVectors - 1]), acc[m][c], 0, 0, 0);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kColumns; ++c)
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(wv[b][m]), as_bf16(xv[b][c][0]), acc[m][c], 0, 0, 0);
-        }
-      }
-  }
-}
-
-__device__ __forceinline__ int expert_of(const FewTokensArgs& a, int route, int routes) {
-  if (route >= routes) return -1;
-  const int64_t e = a.topk_idx[route];
-  return e >= 0 && e < a.num_experts ? static_cast<int>(e) : -1;
-}
-
-// The routes of expert e in order into a wave's own list; returns how many.  The ids come from LDS or memory.
-template <typename Ids>
-__device__ __forceinline__ int collect_routes(const Ids& ids, int routes, int e, uint16_t* list) {
-  const int lane = lane_id();
-  int n = 0;
-  for (int base = 0; base < routes; base += kWave) {
-    const bool match = ids(base + lane) == e;
-    const uint64_t mask = __ballot(match);
-    if (match) list[n + __popcll(mask & lanes_below(lane))] = static_cast<uint16_t>(base + lane);
-    n += __popcll(mask);
-  }
-  __builtin_amdgcn_wave_barrier();
-  return n;
-}
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, kRawBufferFormat);
 }
+__device__ __forceinline__ void wait_lds_and_meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// kColumns blocks of 16 routes from c0 on, through 16 gate and 16 up rows: the waves share out k.
-template <bool kInt8, int kColumns, int kBatch>
-__device__ __forceinline__ void gate_up(const FewTokensArgs& a, int e, int i0, const uint16_t* list, int count, int c0,
-                                        float (&partial)[kFirstWaves][2][4][kWave]) {
-  using C = Chunk<kInt8>;
-  const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) >> 6;
-  const int H = a.hidden, I = a.intermediate;
-  const unsigned char* gate = a.w13 + (static_cast<size_t>(e) * 2 * I + i0) * H * C::kBytes;
-  const __amdgpu_buffer_rsrc_t w[2] = {rows_of(gate, 16 * H * C::kBytes),
-                                       rows_of(gate + static_cast<size_t>(I) * H * C::kBytes, 16 * H * C::kBytes)};
-  int x_at[kColumns];
-#pragma unroll
-  for (int c = 0; c < kColumns; ++c) {
-    const int column = c0 + c * 16 + (lane & 15);
-    x_at[c] = column < count ? list[column] / a.num_topk * H * 2 + (lane >> 4) * C::kLane * 2 : kOutside;
-  }
-  float4v acc[2][kColumns];
-#pragma unroll
-  for (int c = 0; c < kColumns; ++c) acc[0][c] = acc[1][c] = float4v{0, 0, 0, 0};
-  const int chunks = (H + C::kElements - 1) / C::kElements;
-  multiply<kInt8, 2, kColumns, kBatch>(w, (lane & 15) * H * C::kBytes + (lane >> 4) * 16, rows_of(a.x, a.num_tokens * H * 2),
-                                       x_at, chunks * wave / kFirstWaves, chunks * (wave + 1) / kFirstWaves, H, acc);
-#pragma unroll
-  for (int c = 0; c < kColumns; ++c) {
-    if (c0 + c * 16 >= count) break;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      partial[wave][0][i][lane] = acc[0][c][i];
-      partial[wave][1][i][lane] = acc[1][c][i];
+// Who meets whom, made by every workgroup for itself from the ids: `entries` lists the met experts by their
+// first routes, once for every 16 * kColumns of an expert's routes (first route | pass << 10).
+struct Meeting {
+  int16_t* ids;       // [routes] expert of every route, -1 for none
+  uint16_t* entries;  // [routes]
+  int count;
+
+  static constexpr int bytes(int routes) { return routes * 4; }
+
+  // scratch: num_experts words twice.  All threads; ends with the lists visible to all.
+  template <int kColumns>
+  __device__ __forceinline__ void make(const FewTokensArgs& a, int routes, unsigned char* at, int* scratch) {
+    __shared__ int total;
+    ids = reinterpret_cast<int16_t*>(at);
+    entries = reinterpret_cast<uint16_t*>(at) + routes;
+    int* first = scratch;
+    int* met = scratch + a.num_experts;
+    const int t = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
+    for (int e = t; e < a.num_experts; e += threads) {
+      first[e] = 0x7fffffff;
+      met[e] = 0;
     }
-    __syncthreads();
-    // Thread 16 j + n: row n of column j, held by lane 16 (n / 4) + j as value n % 4.
+    wait_lds_and_meet();
+    for (int r = t; r < routes; r += threads) {
+      const int64_t e = a.topk_idx[r];
+      const bool routed = e >= 0 && e < a.num_experts;
+      ids[r] = static_cast<int16_t>(routed ? e : -1);
+      if (routed) {  // the minimum and the sum do not depend on the order of the waves
+        atomicMin(first + e, r);
+        atomicAdd(met + e, 1);
+      }
+    }
+    wait_lds_and_meet();
+    if (t < kWave) {
+      int n = 0;
+      for (int base = 0; base < routes; base += kWave) {
+        const int r = base + t;
+        const int e = r < routes ? ids[r] : -1;
+        const int passes = e >= 0 && first[e] == r ? (met[e] + 16 * kColumns - 1) / (16 * kColumns) : 0;
+        const int upto = wave_inclusive_scan(passes);
+        for (int p = 0; p < passes; ++p) entries[n + upto - passes + p] = static_cast<uint16_t>(r | p << 10);
+        n += wave_read(upto, kWave - 1);
+      }
+      if (t == 0) total = n;
+    }
+    wait_lds_and_meet();
+    count = __builtin_amdgcn_readfirstlane(total);
+  }
+
+  __device__ __forceinline__ int expert(int entry) const {
+    return __builtin_amdgcn_readfirstlane(ids[entries[entry] & 1023]);
+  }
+  // Routes of an entry's pass: lane l gets that of column 16 c + l % 16, -1 for none.  `list` is the wave's own.
+  template <int kColumns>
+  __device__ __forceinline__ void columns(int entry, int routes, uint16_t* list, int (&route)[kColumns]) const {
+    const int lane = lane_id();
+    const int packed = __builtin_amdgcn_readfirstlane(entries[entry]);
+    const int e = __builtin_amdgcn_readfirstlane(ids[packed & 1023]);
+    int rank = -(packed >> 10) * 16 * kColumns;  // of the next match
+    for (int base = packed & 1023 & ~(kWave - 1); base < routes && rank < 16 * kColumns; base += kWave) {
+      const bool match = base + lane < routes && ids[base + lane] == e;
+      const uint64_t mask = __ballot(match);
+      const int at = rank + __popcll(mask & lanes_below(lane));
+      if (match && at >= 0 && at < 16 * kColumns) list[at] = static_cast<uint16_t>(base + lane);
+      rank += __popcll(mask);
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      const int column = c * 16 + (lane & 15);
+      route[c] = column < rank ? list[column] : -1;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// The stream of chunks that a wave works through, item after item (an item: kMatrices blocks of 16 weight rows
+// times the columns of an entry).  kDepth chunks are always on their way: the place of a chunk that was
+// used is filled with the one kDepth further on, also across the end of an item, whose number of chunks
+// is rounded up to a multiple of kDepth (the excess loads nothing).
+template <bool kInt8, int kMatrices, int kColumns, int kDepth>
+struct Stream {
+  using C = Chunk<kInt8>;
+  vec16 w[kDepth][2][kMatrices], x[kDepth][2][kColumns][C::kVectors];
+
+  // Where the loads stand: an item's weights and columns, and the next chunk.
+  const unsigned char* rows[kMatrices];
+  int row_bytes;  // of 16 rows
+  int w_lane, x_at[kColumns], k, k_end;
+
+  __device__ __forceinline__ void load(int slot, __amdgpu_buffer_rsrc_t vectors) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool inside = k + h * C::kPiece < k_end;
+      const int at = inside ? w_lane + k * C::kBytes + h * 16 : kOutside;
+#pragma unroll
+      for (int m = 0; m < kMatrices; ++m)
+        w[slot][h][m] = __builtin_amdgcn_raw_buffer_load_b128(rows_of(rows[m], row_bytes), at, 0, 0);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bool inside = k + h * C::kPiece < k_end;
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) {
+        const int from = inside ? x_at[c] + k * 2 : kOutside;
+#pragma unroll
+        for (int v = 0; v < C::kVectors; ++v)
+          x[slot][h][c][v] = __builtin_amdgcn_raw_buffer_load_b128(vectors, from + 16 * (h * C::kVectors + v), 0, 0);
+      }
+    }
+    k += C::kElements;
+  }
+  __device__ __forceinline__ void use(int slot, float4v (&acc)[kMatrices][kColumns]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int m = 0; m < kMatrices; ++m) {
+        const vec16 v = w[slot][h][m];
+        if constexpr (kInt8) {
+          const bf16x8 w0 = widen(v[0], v[1]), w1 = widen(v[2], v[3]);
+#pragma unroll
+          for (int c = 0; c < kColumns; ++c) {
+            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, as_bf16(x[slot][h][c][0]), acc[m][c], 0, 0, 0);
+            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, as_bf16(x[slot][h][c][C::kVectors - 1]), acc[m][c], 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kColumns; ++c)
+            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(v), as_bf16(x[slot][h][c][0]), acc[m][c], 0, 0, 0);
+        }
+      }
+  }
+};
+
+// Gate and up.  Items are (entry, 16 columns of act); workgroup b takes the b-th contiguous share of them.  The
+// four waves split an item's k and add their sums through LDS.
+template <bool kInt8, int kColumns, int kDepth>
+__global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel(const FewTokensArgs a) {
+  using C = Chunk<kInt8>;
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ float partial[2][kFirstWaves][2][4][kWave];
+  __shared__ uint16_t lists[kFirstWaves][16 * kColumns];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int routes = a.num_tokens * a.num_topk;
+  Meeting meeting;
+  // The experts' words lie where the sums go later: kMaxExperts words twice.
+  static_assert(sizeof(partial) >= 2 * kMaxExperts * sizeof(int), "scratch of the meeting");
+  meeting.make<kColumns>(a, routes, shared, reinterpret_cast<int*>(&partial[0][0][0][0][0]));
+
+  const int H = a.hidden, I = a.intermediate;
+  const int slices = I / 16;
+  const long long items = static_cast<long long>(meeting.count) * slices;
+  const long long workgroups = static_cast<long long>(gridDim.x);
+  const int from = static_cast<int>(items * blockIdx.x / workgroups), to = static_cast<int>(items * (blockIdx.x + 1) / workgroups);
+  if (from >= to) return;
+
+  const int chunks = (H + C::kElements - 1) / C::kElements;
+  const int share = (chunks + kFirstWaves - 1) / kFirstWaves;  // of a wave
+  const int rounds = (share + kDepth - 1) / kDepth;
+  const int k_lane = (lane >> 4) * C::kLane;
+  const int k_begin = share * wave * C::kElements + k_lane;
+  const int share_end = share * (wave + 1) * C::kElements;
+  const int k_stop = share_end < H ? share_end : H;
+
+  const __amdgpu_buffer_rsrc_t vectors = rows_of(a.x, a.num_tokens * H * 2);
+  Stream<kInt8, 2, kColumns, kDepth> s;
+  s.row_bytes = 16 * H * C::kBytes;
+  s.w_lane = (lane & 15) * H * C::kBytes;
+  int next_route[kColumns], route[kColumns];
+  int ahead = from, ahead_entry = -1;  // where the loads stand
+  const auto begin_item = [&]() {
+    if (ahead >= to) {
+      s.k_end = 0;
+      return;
+    }
+    const int entry = ahead / slices;
+    const int e = meeting.expert(entry);
+    if (entry != ahead_entry) {
+      meeting.columns<kColumns>(entry, routes, lists[wave], next_route);
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] / a.num_topk * H * 2 : kOutside;
+      ahead_entry = entry;
+    }
+    s.rows[0] = a.w13 + (static_cast<size_t>(e) * 2 * I + (ahead - entry * slices) * 16) * H * C::kBytes;
+    s.rows[1] = s.rows[0] + static_cast<size_t>(I) * H * C::kBytes;
+    s.k = k_begin;
+    s.k_end = k_stop;
+  };
+  begin_item();
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) s.load(d, vectors);
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
+
+  for (int item = from; item < to; ++item) {
+    float4v acc[2][kColumns];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) acc[0][c] = acc[1][c] = float4v{0, 0, 0, 0};
+    for (int round = 0; round < rounds; ++round) {
+      if (round == rounds - 1) {
+        ++ahead;
+        begin_item();
+      }
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        s.use(d, acc);
+        s.load(d, vectors);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    const int entry = item / slices;
+    const int e = meeting.expert(entry), i0 = (item - entry * slices) * 16;
+    // Thread 16 j + n adds up row n of column j, held by lane 16 (n / 4) + j as value n % 4.
     const int n = static_cast<int>(threadIdx.x) & 15, j = static_cast<int>(threadIdx.x) >> 4;
-    const int column = c0 + c * 16 + j;
-    if (column < count) {
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      float(&sums)[kFirstWaves][2][4][kWave] = partial[(item * kColumns + c) & 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sums[wave][0][i][lane] = acc[0][c][i];
+        sums[wave][1][i][lane] = acc[1][c][i];
+      }
+      wait_lds_and_meet();
+      const int column_route = __shfl(route[c], j);
       float g = 0.0f, u = 0.0f;
 #pragma unroll
       for (int v = 0; v < kFirstWaves; ++v) {
-        g += partial[v][0][n & 3][(n >> 2) * 16 + j];
-        u += partial[v][1][n & 3][(n >> 2) * 16 + j];
+        g += sums[v][0][n & 3][(n >> 2) * 16 + j];
+        u += sums[v][1][n & 3][(n >> 2) * 16 + j];
       }
-      if constexpr (kInt8) {
-        const float* scales = a.w13_scales + static_cast<size_t>(e) * 2 * I + i0 + n;
-        g *= scales[0];
-        u *= scales[I];
+      if (column_route >= 0) {
+        if constexpr (kInt8) {
+          const float* scales = a.w13_scales + static_cast<size_t>(e) * 2 * I + i0 + n;
+          g *= scales[0];
+          u *= scales[I];
+        }
+        a.act[static_cast<size_t>(column_route) * I + i0 + n] =
+            static_cast<uint16_t>(f32_to_bf16_bits(g / (1.0f + __expf(-g)) * u));
       }
-      a.act[static_cast<size_t>(list[column]) * I + i0 + n] =
-          static_cast<uint16_t>(f32_to_bf16_bits(g / (1.0f + __expf(-g)) * u));
     }
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
   }
 }
 
-// Workgroup (s, r): 16 columns of act for the expert of route r, if r is that expert's first route.
-template <bool kInt8>
-__global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel(const FewTokensArgs a) {
-  __shared__ uint16_t lists[kFirstWaves][kFewRoutes];
-  __shared__ float partial[kFirstWaves][2][4][kWave];
-  const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const int routes = a.num_tokens * a.num_topk;
-  const int r = static_cast<int>(blockIdx.y);
-  const int e = expert_of(a, r, routes);
-  uint16_t* list = lists[wave];  // every wave makes its own: no barrier before the first load
-  const int count = e < 0 ? 0 : collect_routes([&](int q) { return expert_of(a, q, routes); }, routes, e, list);
-  const bool leads = count > 0 && list[0] == r;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.leaders[r] = leads ? 1 : 0;
-  if (!leads) return;
-  const int i0 = static_cast<int>(blockIdx.x) * 16;
-  for (int c0 = 0; c0 < count;) {
-    const int left = count - c0;
-    if (left <= 16) {
-      gate_up<kInt8, 1, 4>(a, e, i0, list, count, c0, partial);
-      c0 += 16;
-    } else if (left <= 32) {
-      gate_up<kInt8, 2, 2>(a, e, i0, list, count, c0, partial);
-      c0 += 32;
-    } else {
-      gate_up<kInt8, 4, 1>(a, e, i0, list, count, c0, partial);
-      c0 += 64;
-    }
-  }
-}
-
-// kColumns blocks of 16 routes from c0 on, through 16 rows of the down weights over chunks [begin, end).
-template <bool kInt8, int kColumns, int kBatch>
-__device__ __forceinline__ void down(const FewTokensArgs& a, int e, int h0, const uint16_t* list, int count, int c0, int begin,
-                                     int end, float* y) {
-  using C = Chunk<kInt8>;
-  const int lane = lane_id();
-  const int H = a.hidden, I = a.intermediate;
-  const __amdgpu_buffer_rsrc_t w[1] = {rows_of(a.w2 + (static_cast<size_t>(e) * H + h0) * I * C::kBytes, 16 * I * C::kBytes)};
-  int x_at[kColumns];
-#pragma unroll
-  for (int c = 0; c < kColumns; ++c) {
-    const int column = c0 + c * 16 + (lane & 15);
-    x_at[c] = column < count ? list[column] * I * 2 + (lane >> 4) * C::kLane * 2 : kOutside;
-  }
-  float4v acc[1][kColumns];
-#pragma unroll
-  for (int c = 0; c < kColumns; ++c) acc[0][c] = float4v{0, 0, 0, 0};
-  multiply<kInt8, 1, kColumns, kBatch>(w, (lane & 15) * I * C::kBytes + (lane >> 4) * 16,
-                                       rows_of(a.act, a.num_tokens * a.num_topk * I * 2), x_at, begin, end, I, acc);
-  float scales[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-  if constexpr (kInt8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) scales[i] = a.w2_scales[static_cast<size_t>(e) * H + h0 + (lane >> 4) * 4 + i];
-  }
-#pragma unroll
-  for (int c = 0; c < kColumns; ++c) {
-    const int column = c0 + c * 16 + (lane & 15);
-    if (column < count) {
-      float* out = y + list[column] * 16 + (lane >> 4) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[i] = acc[0][c][i] * scales[i];
-    }
-  }
-}
-
-// Workgroup h: 16 columns of the output for every token.  The waves share out the met experts (and, with
-// fewer experts than waves, ranges of the intermediate axis); y[split][route][16] collects their products.
-template <bool kInt8>
+// Down.  Workgroup h: 16 columns of the output for every token.  Items are the entries (with fewer of them than
+// waves, shares of their k); wave w takes items w, w + 8, ...  y[split][route][16] collects the products.
+template <bool kInt8, int kColumns, int kDepth>
 __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(const FewTokensArgs a, const int splits) {
-  extern __shared__ float y[];
+  using C = Chunk<kInt8>;
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ uint16_t lists[kSecondWaves][16 * kColumns];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int routes = a.num_tokens * a.num_topk;
-  int* ids = reinterpret_cast<int*>(y + splits * routes * 16);
-  uint16_t* leaders = reinterpret_cast<uint16_t*>(ids + routes);
-  uint16_t* lists = leaders + routes;  // [kSecondWaves][routes]
-  __shared__ int met;
-  const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) >> 6;
-  for (int r = static_cast<int>(threadIdx.x); r < routes; r += kSecondThreads) ids[r] = expert_of(a, r, routes);
-  if (wave == kSecondWaves - 1) {  // the first route of every met expert, in order
-    const int n = collect_routes([&](int r) { return r < routes ? a.leaders[r] : 0; }, routes, 1, leaders);
-    if (lane == 0) met = n;
-  }
-  __syncthreads();
+  Meeting meeting;
+  float* y = reinterpret_cast<float*>(shared + ((Meeting::bytes(routes) + 15) & ~15));
+  meeting.make<kColumns>(a, routes, shared, reinterpret_cast<int*>(y));  // y's place is the scratch
 
+  const int H = a.hidden, I = a.intermediate;
   const int h0 = static_cast<int>(blockIdx.x) * 16;
-  const int chunks = (a.intermediate + Chunk<kInt8>::kElements - 1) / Chunk<kInt8>::kElements;
-  uint16_t* list = lists + wave * routes;
-  for (int item = wave; item < met * splits; item += kSecondWaves) {
-    const int leader = item / splits, split = item - leader * splits;
-    const int e = ids[leaders[leader]];
-    const int count = collect_routes([&](int r) { return r < routes ? ids[r] : -1; }, routes, e, list);
-    const int begin = chunks * split / splits, end = chunks * (split + 1) / splits;
-    float* to = y + split * routes * 16;
-    for (int c0 = 0; c0 < count;) {
-      const int left = count - c0;
-      if (left <= 16) {
-        down<kInt8, 1, 8>(a, e, h0, list, count, c0, begin, end, to);
-        c0 += 16;
-      } else if (left <= 32) {
-        down<kInt8, 2, 4>(a, e, h0, list, count, c0, begin, end, to);
-        c0 += 32;
-      } else {
-        down<kInt8, 4, 2>(a, e, h0, list, count, c0, begin, end, to);
-        c0 += 64;
+  const int items = meeting.count * splits;
+  const int chunks = (I + C::kElements - 1) / C::kElements;
+  const int share = (chunks + splits - 1) / splits;
+  const int rounds = (share + kDepth - 1) / kDepth;
+  const int k_lane = (lane >> 4) * C::kLane;
+
+  const __amdgpu_buffer_rsrc_t vectors = rows_of(a.act, routes * I * 2);
+  Stream<kInt8, 1, kColumns, kDepth> s;
+  s.row_bytes = 16 * I * C::kBytes;
+  s.w_lane = (lane & 15) * I * C::kBytes;
+  int next_route[kColumns], route[kColumns];
+  int ahead = wave;
+  const auto begin_item = [&]() {
+    if (ahead >= items) {
+      s.k_end = 0;
+      return;
+    }
+    const int entry = ahead / splits, split = ahead - entry * splits;
+    meeting.columns<kColumns>(entry, routes, lists[wave], next_route);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] * I * 2 : kOutside;
+    s.rows[0] = a.w2 + (static_cast<size_t>(meeting.expert(entry)) * H + h0) * I * C::kBytes;
+    const int end = share * (split + 1) * C::kElements;
+    s.k = share * split * C::kElements + k_lane;
+    s.k_end = end < I ? end : I;
+  };
+  if (wave < items) {
+    begin_item();
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) s.load(d, vectors);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
+  }
+  for (int item = wave; item < items; item += kSecondWaves) {
+    float4v acc[1][kColumns];
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) acc[0][c] = float4v{0, 0, 0, 0};
+    for (int round = 0; round < rounds; ++round) {
+      if (round == rounds - 1) {
+        ahead += kSecondWaves;
+        begin_item();
+      }
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        s.use(d, acc);
+        s.load(d, vectors);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    const int entry = item / splits, split = item - entry * splits;
+    const int n = (lane >> 4) * 4;
+    float scales[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    if constexpr (kInt8) {
+      const float4 of = *reinterpret_cast<const float4*>(a.w2_scales + static_cast<size_t>(meeting.expert(entry)) * H + h0 + n);
+      scales[0] = of.x, scales[1] = of.y, scales[2] = of.z, scales[3] = of.w;
+    }
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      if (route[c] >= 0) {
+        float4 out = {acc[0][c][0] * scales[0], acc[0][c][1] * scales[1], acc[0][c][2] * scales[2], acc[0][c][3] * scales[3]};
+        *reinterpret_cast<float4*>(y + (split * routes + route[c]) * 16 + n) = out;
+      }
+      route[c] = next_route[c];
+    }
   }
-  __syncthreads();
+  wait_lds_and_meet();
   for (int j = static_cast<int>(threadIdx.x); j < a.num_tokens * 16; j += kSecondThreads) {
     const int t = j >> 4, c = j & 15;
     float sum = 0.0f;
     for (int k = 0; k < a.num_topk; ++k) {
       const int r = t * a.num_topk + k;
-      if (ids[r] < 0) continue;
+      if (meeting.ids[r] < 0) continue;
       float v = 0.0f;
-      for (int s = 0; s < splits; ++s) v += y[(s * routes + r) * 16 + c];
+      for (int split = 0; split < splits; ++split) v += y[(split * routes + r) * 16 + c];
       sum = __builtin_fmaf(a.topk_weights != nullptr ? a.topk_weights[r] : 1.0f, v, sum);
     }
-    const size_t o = static_cast<size_t>(t) * a.hidden + h0 + c;
+    const size_t o = static_cast<size_t>(t) * H + h0 + c;
     if (a.bias_0 != nullptr) sum += bf16_lo(a.bias_0[o]);
     if (a.bias_1 != nullptr) sum += bf16_lo(a.bias_1[o]);
     a.combined_x[o] = static_cast<uint16_t>(f32_to_bf16_bits(sum));
   }
 }
 
-template <bool kInt8>
+template <bool kInt8, int kColumns, int kFirstDepth, int kSecondDepth>
 hipError_t launch_few_tokens_as(const FewTokensArgs& a, hipStream_t stream) {
   const int routes = a.num_tokens * a.num_topk;
-  hipLaunchKernelGGL((ep_few_tokens_gate_up_kernel<kInt8>),
-                     dim3(static_cast<unsigned>(a.intermediate / 16), static_cast<unsigned>(routes)), dim3(kFirstThreads), 0,
-                     stream, a);
-  hipError_t e = hipGetLastError();
+  DeviceTraits dev{};
+  hipError_t e = device_traits(stream, &dev);
+  if (e != hipSuccess) return e;
+  // As many workgroups as are resident at once, or items.
+  const long long items = static_cast<long long>(routes) * (a.intermediate / 16);
+  const long long resident = 4LL * dev.compute_units;
+  const unsigned first = static_cast<unsigned>(items < resident ? items : resident);
+  const size_t lists = (static_cast<size_t>(Meeting::bytes(routes)) + 15) & ~static_cast<size_t>(15);
+  hipLaunchKernelGGL((ep_few_tokens_gate_up_kernel<kInt8, kColumns, kFirstDepth>), dim3(first), dim3(kFirstThreads), lists, stream, a);
+  e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int splits = routes >= kSecondWaves ? 1 : kSecondWaves / routes;
-  const size_t lds = static_cast<size_t>(splits) * routes * 16 * sizeof(float) + routes * sizeof(int) +
-                     static_cast<size_t>(routes) * (1 + kSecondWaves) * sizeof(uint16_t);
-  if (lds > 64 * 1024) {
+  const size_t sums = static_cast<size_t>(splits) * routes * 16 * sizeof(float);
+  const size_t scratch = static_cast<size_t>(a.num_experts) * 2 * sizeof(int);
+  const size_t lds = lists + (sums > scratch ? sums : scratch);
+  if (lds > 60 * 1024) {
     // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
     int ordinal = 0;
     e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
@@ -325,22 +434,30 @@ hipError_t launch_few_tokens_as(const FewTokensArgs& a, hipStream_t stream) {
     static std::atomic<int> lds_limit_raised[kMaxDevices];
     if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
     if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kColumns, kSecondDepth>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
       if (e != hipSuccess) return e;
       lds_limit_raised[ordinal].store(1, std::memory_order_release);
     }
   }
-  hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8>), dim3(static_cast<unsigned>(a.hidden / 16)), dim3(kSecondThreads), lds,
-                     stream, a, splits);
+  hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8, kColumns, kSecondDepth>), dim3(static_cast<unsigned>(a.hidden / 16)),
+                     dim3(kSecondThreads), lds, stream, a, splits);
   return hipGetLastError();
+}
+
+template <bool kInt8>
+hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
+  // Columns of a pass by the routes an expert gets on average: a pass reads the weights once more.
+  const int average = a.num_tokens * a.num_topk / a.num_experts;
+  if (average <= 8) return launch_few_tokens_as<kInt8, 1, 2, 4>(a, stream);
+  return launch_few_tokens_as<kInt8, 4, 1, kInt8 ? 1 : 2>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_few_tokens(const FewTokensArgs& a, hipStream_t stream) {
   if (a.num_tokens == 0) return hipSuccess;
-  return a.w13_scales != nullptr ? launch_few_tokens_as<true>(a, stream) : launch_few_tokens_as<false>(a, stream);
+  return a.w13_scales != nullptr ? launch_few_tokens_with<true>(a, stream) : launch_few_tokens_with<false>(a, stream);
 }
 
 }  // namespace mi_ep
