@@ -57,6 +57,8 @@ struct Chunk {
   static constexpr int kLane = 2 * kPiece;        // of a lane
   static constexpr int kElements = 4 * kLane;     // of k
   static constexpr int kVectors = kInt8 ? 2 : 1;  // 16-byte bf16 loads of a column for a load of weights
+  static constexpr int kAll = 2 * kVectors;       // and for a lane's whole chunk
+  static constexpr int kFoldColumns = 16 / kAll;  // columns of a folded load
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int bytes) {
@@ -65,20 +67,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int 
 __device__ __forceinline__ void wait_lds_and_meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Who meets whom, made by every workgroup for itself from the ids: `entries` lists the met experts by their
-// first routes, once for every 16 * kColumns of an expert's routes (first route | pass << 10).
+// first routes, once for every kPass of an expert's routes (first route | pass << 10).
+template <int kPass>
 struct Meeting {
+  uint32_t* entries;  // [routes]
   int16_t* ids;       // [routes] expert of every route, -1 for none
-  uint16_t* entries;  // [routes]
   int count;
 
-  static constexpr int bytes(int routes) { return routes * 4; }
+  static constexpr size_t bytes(int routes) { return (static_cast<size_t>(routes) * 6 + 15) & ~static_cast<size_t>(15); }
 
   // scratch: num_experts words twice.  All threads; ends with the lists visible to all.
-  template <int kColumns>
   __device__ __forceinline__ void make(const FewTokensArgs& a, int routes, unsigned char* at, int* scratch) {
     __shared__ int total;
-    ids = reinterpret_cast<int16_t*>(at);
-    entries = reinterpret_cast<uint16_t*>(at) + routes;
+    entries = reinterpret_cast<uint32_t*>(at);
+    ids = reinterpret_cast<int16_t*>(entries + routes);
     int* first = scratch;
     int* met = scratch + a.num_experts;
     const int t = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
@@ -102,9 +104,9 @@ struct Meeting {
       for (int base = 0; base < routes; base += kWave) {
         const int r = base + t;
         const int e = r < routes ? ids[r] : -1;
-        const int passes = e >= 0 && first[e] == r ? (met[e] + 16 * kColumns - 1) / (16 * kColumns) : 0;
+        const int passes = e >= 0 && first[e] == r ? (met[e] + kPass - 1) / kPass : 0;
         const int upto = wave_inclusive_scan(passes);
-        for (int p = 0; p < passes; ++p) entries[n + upto - passes + p] = static_cast<uint16_t>(r | p << 10);
+        for (int p = 0; p < passes; ++p) entries[n + upto - passes + p] = static_cast<uint32_t>(r | p << 10);
         n += wave_read(upto, kWave - 1);
       }
       if (t == 0) total = n;
@@ -116,26 +118,25 @@ struct Meeting {
   __device__ __forceinline__ int expert(int entry) const {
     return __builtin_amdgcn_readfirstlane(ids[entries[entry] & 1023]);
   }
-  // Routes of an entry's pass: lane l gets that of column 16 c + l % 16, -1 for none.  `list` is the wave's own.
+  // An entry's routes into the wave's own list; then the lane's routes are those of columns column[c], -1 where the
+  // pass has none.
   template <int kColumns>
-  __device__ __forceinline__ void columns(int entry, int routes, uint16_t* list, int (&route)[kColumns]) const {
+  __device__ __forceinline__ void columns(int entry, int routes, uint16_t* list, const int (&column)[kColumns],
+                                          int (&route)[kColumns]) const {
     const int lane = lane_id();
-    const int packed = __builtin_amdgcn_readfirstlane(entries[entry]);
+    const int packed = __builtin_amdgcn_readfirstlane(static_cast<int>(entries[entry]));
     const int e = __builtin_amdgcn_readfirstlane(ids[packed & 1023]);
-    int rank = -(packed >> 10) * 16 * kColumns;  // of the next match
-    for (int base = packed & 1023 & ~(kWave - 1); base < routes && rank < 16 * kColumns; base += kWave) {
+    int rank = -(packed >> 10) * kPass;  // of the next match
+    for (int base = packed & 1023 & ~(kWave - 1); base < routes && rank < kPass; base += kWave) {
       const bool match = base + lane < routes && ids[base + lane] == e;
       const uint64_t mask = __ballot(match);
       const int at = rank + __popcll(mask & lanes_below(lane));
-      if (match && at >= 0 && at < 16 * kColumns) list[at] = static_cast<uint16_t>(base + lane);
+      if (match && at >= 0 && at < kPass) list[at] = static_cast<uint16_t>(base + lane);
       rank += __popcll(mask);
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) {
-      const int column = c * 16 + (lane & 15);
-      route[c] = column < rank ? list[column] : -1;
-    }
+    for (int c = 0; c < kColumns; ++c) route[c] = column[c] < rank ? list[column[c]] : -1;
     __builtin_amdgcn_wave_barrier();
   }
 };
@@ -144,15 +145,23 @@ struct Meeting {
 // times the columns of an entry).  kDepth chunks are always on their way: the place of a chunk that was
 // used is filled with the one kDepth further on, also across the end of an item, whose number of chunks
 // is rounded up to a multiple of kDepth (the excess loads nothing).
-template <bool kInt8, int kMatrices, int kColumns, int kDepth>
+//
+// Folded (passes of no more than kFoldColumns columns): most of a column load's 16 columns would be empty, so one
+// load fetches all of a lane's kAll vectors for kFoldColumns columns, vector v in columns v * kFoldColumns and
+// on.  Product v then has its sums in those columns of its own accumulator, and the accumulators are put
+// together when the item ends.
+template <bool kInt8, int kMatrices, int kColumns, int kDepth, bool kFold>
 struct Stream {
   using C = Chunk<kInt8>;
-  vec16 w[kDepth][2][kMatrices], x[kDepth][2][kColumns][C::kVectors];
+  static_assert(!kFold || kColumns == 1, "only a single block of columns folds");
+  static constexpr int kSums = kFold ? C::kAll : kColumns;
+  vec16 w[kDepth][2][kMatrices], x[kDepth][kFold ? 1 : 2][kColumns][kFold ? 1 : C::kVectors];
 
   // Where the loads stand: an item's weights and columns, and the next chunk.
   const unsigned char* rows[kMatrices];
   int row_bytes;  // of 16 rows
   int w_lane, x_at[kColumns], k, k_end;
+
 
   __device__ __forceinline__ void load(int slot, __amdgpu_buffer_rsrc_t vectors) {
 #pragma unroll
@@ -163,37 +172,46 @@ struct Stream {
       for (int m = 0; m < kMatrices; ++m)
         w[slot][h][m] = __builtin_amdgcn_raw_buffer_load_b128(rows_of(rows[m], row_bytes), at, 0, 0);
     }
+    if constexpr (kFold) {  // x_at includes the lane's vector
+      const int v = (lane_id() & 15) / C::kFoldColumns;
+      x[slot][0][0][0] = __builtin_amdgcn_raw_buffer_load_b128(
+          vectors, k + v / C::kVectors * C::kPiece < k_end ? x_at[0] + k * 2 : kOutside, 0, 0);
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool inside = k + h * C::kPiece < k_end;
+      for (int h = 0; h < 2; ++h) {
+        const bool inside = k + h * C::kPiece < k_end;
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) {
-        const int from = inside ? x_at[c] + k * 2 : kOutside;
+        for (int c = 0; c < kColumns; ++c) {
+          const int from = inside ? x_at[c] + k * 2 : kOutside;
 #pragma unroll
-        for (int v = 0; v < C::kVectors; ++v)
-          x[slot][h][c][v] = __builtin_amdgcn_raw_buffer_load_b128(vectors, from + 16 * (h * C::kVectors + v), 0, 0);
+          for (int v = 0; v < C::kVectors; ++v)
+            x[slot][h][c][v] = __builtin_amdgcn_raw_buffer_load_b128(vectors, from + 16 * (h * C::kVectors + v), 0, 0);
+        }
       }
     }
     k += C::kElements;
   }
-  __device__ __forceinline__ void use(int slot, float4v (&acc)[kMatrices][kColumns]) const {
+  __device__ __forceinline__ void use(int slot, float4v (&acc)[kMatrices][kSums]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int m = 0; m < kMatrices; ++m) {
-        const vec16 v = w[slot][h][m];
+        const vec16 packed = w[slot][h][m];
+        bf16x8 rows16[C::kVectors];
         if constexpr (kInt8) {
-          const bf16x8 w0 = widen(v[0], v[1]), w1 = widen(v[2], v[3]);
+          rows16[0] = widen(packed[0], packed[1]);
+          rows16[1] = widen(packed[2], packed[3]);
+        } else {
+          rows16[0] = as_bf16(packed);
+        }
+#pragma unroll
+        for (int v = 0; v < C::kVectors; ++v)
 #pragma unroll
           for (int c = 0; c < kColumns; ++c) {
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, as_bf16(x[slot][h][c][0]), acc[m][c], 0, 0, 0);
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, as_bf16(x[slot][h][c][C::kVectors - 1]), acc[m][c], 0, 0, 0);
+            const int sum = kFold ? h * C::kVectors + v : c;
+            const bf16x8 columns16 = as_bf16(kFold ? x[slot][0][0][0] : x[slot][kFold ? 0 : h][c][kFold ? 0 : v]);
+            acc[m][sum] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows16[v], columns16, acc[m][sum], 0, 0, 0);
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kColumns; ++c)
-            acc[m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(v), as_bf16(x[slot][h][c][0]), acc[m][c], 0, 0, 0);
-        }
       }
   }
 };
@@ -208,10 +226,10 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
   __shared__ uint16_t lists[kFirstWaves][16 * kColumns];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int routes = a.num_tokens * a.num_topk;
-  Meeting meeting;
+  Meeting<16 * kColumns> meeting;
   // The experts' words lie where the sums go later: kMaxExperts words twice.
   static_assert(sizeof(partial) >= 2 * kMaxExperts * sizeof(int), "scratch of the meeting");
-  meeting.make<kColumns>(a, routes, shared, reinterpret_cast<int*>(&partial[0][0][0][0][0]));
+  meeting.make(a, routes, shared, reinterpret_cast<int*>(&partial[0][0][0][0][0]));
 
   const int H = a.hidden, I = a.intermediate;
   const int slices = I / 16;
@@ -229,10 +247,12 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
   const int k_stop = share_end < H ? share_end : H;
 
   const __amdgpu_buffer_rsrc_t vectors = rows_of(a.x, a.num_tokens * H * 2);
-  Stream<kInt8, 2, kColumns, kDepth> s;
+  Stream<kInt8, 2, kColumns, kDepth, false> s;
   s.row_bytes = 16 * H * C::kBytes;
   s.w_lane = (lane & 15) * H * C::kBytes;
-  int next_route[kColumns], route[kColumns];
+  int column[kColumns], next_route[kColumns], route[kColumns];
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) column[c] = c * 16 + (lane & 15);
   int ahead = from, ahead_entry = -1;  // where the loads stand
   const auto begin_item = [&]() {
     if (ahead >= to) {
@@ -242,7 +262,7 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
     const int entry = ahead / slices;
     const int e = meeting.expert(entry);
     if (entry != ahead_entry) {
-      meeting.columns<kColumns>(entry, routes, lists[wave], next_route);
+      meeting.template columns<kColumns>(entry, routes, lists[wave], column, next_route);
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] / a.num_topk * H * 2 : kOutside;
       ahead_entry = entry;
@@ -311,16 +331,17 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
 
 // Down.  Workgroup h: 16 columns of the output for every token.  Items are the entries (with fewer of them than
 // waves, shares of their k); wave w takes items w, w + 8, ...  y[split][route][16] collects the products.
-template <bool kInt8, int kColumns, int kDepth>
+template <bool kInt8, int kColumns, int kDepth, bool kFold>
 __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(const FewTokensArgs a, const int splits) {
   using C = Chunk<kInt8>;
   extern __shared__ __align__(16) unsigned char shared[];
-  __shared__ uint16_t lists[kSecondWaves][16 * kColumns];
+  constexpr int kPass = kFold ? C::kFoldColumns : 16 * kColumns;
+  __shared__ uint16_t lists[kSecondWaves][kPass];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int routes = a.num_tokens * a.num_topk;
-  Meeting meeting;
-  float* y = reinterpret_cast<float*>(shared + ((Meeting::bytes(routes) + 15) & ~15));
-  meeting.make<kColumns>(a, routes, shared, reinterpret_cast<int*>(y));  // y's place is the scratch
+  Meeting<kPass> meeting;
+  float* y = reinterpret_cast<float*>(shared + Meeting<kPass>::bytes(routes));
+  meeting.make(a, routes, shared, reinterpret_cast<int*>(y));  // y's place is the scratch
 
   const int H = a.hidden, I = a.intermediate;
   const int h0 = static_cast<int>(blockIdx.x) * 16;
@@ -331,10 +352,14 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
   const int k_lane = (lane >> 4) * C::kLane;
 
   const __amdgpu_buffer_rsrc_t vectors = rows_of(a.act, routes * I * 2);
-  Stream<kInt8, 1, kColumns, kDepth> s;
+  Stream<kInt8, 1, kColumns, kDepth, kFold> s;
+  constexpr int kSums = Stream<kInt8, 1, kColumns, kDepth, kFold>::kSums;
   s.row_bytes = 16 * I * C::kBytes;
   s.w_lane = (lane & 15) * I * C::kBytes;
-  int next_route[kColumns], route[kColumns];
+  int column[kColumns], next_route[kColumns], route[kColumns];
+#pragma unroll
+  for (int c = 0; c < kColumns; ++c) column[c] = kFold ? lane & (C::kFoldColumns - 1) : c * 16 + (lane & 15);
+  const int vector_at = kFold ? (lane & 15) / C::kFoldColumns * 16 : 0;
   int ahead = wave;
   const auto begin_item = [&]() {
     if (ahead >= items) {
@@ -342,9 +367,9 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
       return;
     }
     const int entry = ahead / splits, split = ahead - entry * splits;
-    meeting.columns<kColumns>(entry, routes, lists[wave], next_route);
+    meeting.template columns<kColumns>(entry, routes, lists[wave], column, next_route);
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] * I * 2 : kOutside;
+    for (int c = 0; c < kColumns; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] * I * 2 + vector_at : kOutside;
     s.rows[0] = a.w2 + (static_cast<size_t>(meeting.expert(entry)) * H + h0) * I * C::kBytes;
     const int end = share * (split + 1) * C::kElements;
     s.k = share * split * C::kElements + k_lane;
@@ -358,9 +383,9 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
     for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
   }
   for (int item = wave; item < items; item += kSecondWaves) {
-    float4v acc[1][kColumns];
+    float4v acc[1][kSums];
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) acc[0][c] = float4v{0, 0, 0, 0};
+    for (int c = 0; c < kSums; ++c) acc[0][c] = float4v{0, 0, 0, 0};
     for (int round = 0; round < rounds; ++round) {
       if (round == rounds - 1) {
         ahead += kSecondWaves;
@@ -373,6 +398,18 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    float4v sum[kColumns];
+    if constexpr (kFold) {
+      sum[0] = acc[0][0];
+#pragma unroll
+      for (int v = 1; v < kSums; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[0][i] += __shfl(acc[0][v][i], (lane & 48) + v * C::kFoldColumns + column[0]);
+      if ((lane & 15) >= C::kFoldColumns) route[0] = -1;  // lanes that held other vectors of the same columns
+    } else {
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) sum[c] = acc[0][c];
+    }
     const int entry = item / splits, split = item - entry * splits;
     const int n = (lane >> 4) * 4;
     float scales[4] = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -383,7 +420,7 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) {
       if (route[c] >= 0) {
-        float4 out = {acc[0][c][0] * scales[0], acc[0][c][1] * scales[1], acc[0][c][2] * scales[2], acc[0][c][3] * scales[3]};
+        const float4 out = {sum[c][0] * scales[0], sum[c][1] * scales[1], sum[c][2] * scales[2], sum[c][3] * scales[3]};
         *reinterpret_cast<float4*>(y + (split * routes + route[c]) * 16 + n) = out;
       }
       route[c] = next_route[c];
@@ -407,50 +444,58 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
   }
 }
 
-template <bool kInt8, int kColumns, int kFirstDepth, int kSecondDepth>
-hipError_t launch_few_tokens_as(const FewTokensArgs& a, hipStream_t stream) {
+template <bool kInt8, int kColumns, int kDepth>
+hipError_t launch_gate_up(const FewTokensArgs& a, hipStream_t stream) {
   const int routes = a.num_tokens * a.num_topk;
   DeviceTraits dev{};
-  hipError_t e = device_traits(stream, &dev);
+  const hipError_t e = device_traits(stream, &dev);
   if (e != hipSuccess) return e;
   // As many workgroups as are resident at once, or items.
   const long long items = static_cast<long long>(routes) * (a.intermediate / 16);
   const long long resident = 4LL * dev.compute_units;
-  const unsigned first = static_cast<unsigned>(items < resident ? items : resident);
-  const size_t lists = (static_cast<size_t>(Meeting::bytes(routes)) + 15) & ~static_cast<size_t>(15);
-  hipLaunchKernelGGL((ep_few_tokens_gate_up_kernel<kInt8, kColumns, kFirstDepth>), dim3(first), dim3(kFirstThreads), lists, stream, a);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((ep_few_tokens_gate_up_kernel<kInt8, kColumns, kDepth>),
+                     dim3(static_cast<unsigned>(items < resident ? items : resident)), dim3(kFirstThreads),
+                     Meeting<16 * kColumns>::bytes(routes), stream, a);
+  return hipGetLastError();
+}
+
+template <bool kInt8, int kColumns, int kDepth, bool kFold>
+hipError_t launch_down(const FewTokensArgs& a, hipStream_t stream) {
+  const int routes = a.num_tokens * a.num_topk;
   const int splits = routes >= kSecondWaves ? 1 : kSecondWaves / routes;
   const size_t sums = static_cast<size_t>(splits) * routes * 16 * sizeof(float);
   const size_t scratch = static_cast<size_t>(a.num_experts) * 2 * sizeof(int);
-  const size_t lds = lists + (sums > scratch ? sums : scratch);
+  const size_t lds = Meeting<1>::bytes(routes) + (sums > scratch ? sums : scratch);
   if (lds > 60 * 1024) {
     // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
     int ordinal = 0;
-    e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
+    hipError_t e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
     if (e != hipSuccess) return e;
     constexpr int kMaxDevices = 64;
     static std::atomic<int> lds_limit_raised[kMaxDevices];
     if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
     if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kColumns, kSecondDepth>),
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kColumns, kDepth, kFold>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
       if (e != hipSuccess) return e;
       lds_limit_raised[ordinal].store(1, std::memory_order_release);
     }
   }
-  hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8, kColumns, kSecondDepth>), dim3(static_cast<unsigned>(a.hidden / 16)),
+  hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8, kColumns, kDepth, kFold>), dim3(static_cast<unsigned>(a.hidden / 16)),
                      dim3(kSecondThreads), lds, stream, a, splits);
   return hipGetLastError();
 }
 
 template <bool kInt8>
 hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
-  // Columns of a pass by the routes an expert gets on average: a pass reads the weights once more.
-  const int average = a.num_tokens * a.num_topk / a.num_experts;
-  if (average <= 8) return launch_few_tokens_as<kInt8, 1, 2, 4>(a, stream);
-  return launch_few_tokens_as<kInt8, 4, 1, kInt8 ? 1 : 2>(a, stream);
+  // Columns of a pass by the routes that an expert gets on average: every further pass reads its weights again.
+  const int routes = a.num_tokens * a.num_topk;
+  const bool many = routes > 8 * a.num_experts;
+  const hipError_t e = many ? launch_gate_up<kInt8, 4, 1>(a, stream) : launch_gate_up<kInt8, 1, 2>(a, stream);
+  if (e != hipSuccess) return e;
+  if (many) return launch_down<kInt8, 4, kInt8 ? 1 : 2, false>(a, stream);
+  if (routes > (kInt8 ? 2 : 4) * a.num_experts) return launch_down<kInt8, 1, 4, false>(a, stream);
+  return launch_down<kInt8, 1, 4, true>(a, stream);
 }
 
 }  // namespace
