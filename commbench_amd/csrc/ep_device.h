@@ -231,6 +231,7 @@ struct DequantizeArgs {
   long long scales_row_stride, scales_hidden_stride;
   int num_rows;
   int row_vecs;
+  bool stream_output;  // set by the launcher
 };
 hipError_t launch_dequantize_rows(const DequantizeArgs& a, int format, hipStream_t stream);
 
@@ -386,6 +387,17 @@ __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return (f32_to_bf16_bits(lo) & 0xffffu) | (f32_to_bf16_bits(hi) << 16);
+}
+// The same in the conversion instruction, for two values at a time.
+__device__ __forceinline__ uint32_t to_bf16_pair(float lo, float hi) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  union {
+    bf16x2 b;
+    uint32_t u;
+  } out;
+  out.b = __builtin_convertvector((float2v{lo, hi}), bf16x2);
+  return out.u;
 }
 #endif
 

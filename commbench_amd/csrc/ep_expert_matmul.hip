@@ -54,18 +54,6 @@ __device__ __forceinline__ int4v descriptor_of(const void* base, int bytes) {
                kRawBufferFormat};
 }
 
-// Two fp32 values as packed bf16, rounded to nearest even in one instruction.
-__device__ __forceinline__ uint32_t to_bf16_pair(float lo, float hi) {
-  typedef float float2v __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  union {
-    bf16x2 b;
-    uint32_t u;
-  } out;
-  out.b = __builtin_convertvector((float2v{lo, hi}), bf16x2);
-  return out.u;
-}
-
 // The byte address in LDS of a pointer into it.
 __device__ __forceinline__ int lds_address(const unsigned char* p) {
   return static_cast<int>((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p);

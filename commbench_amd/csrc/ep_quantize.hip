@@ -51,15 +51,13 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {
 
 // y / scale, correctly rounded: with r the rounded reciprocal of the scale, y * r corrected once by its
 // own remainder (Markstein) is the rounded quotient as long as nothing leaves the normal range, which
-// scales from 2^-100 on guarantee for every quotient that matters (larger than 2^-20); smaller or
-// non-finite scales divide.
+// scales from 2^-100 on guarantee for every quotient that matters (larger than 2^-20).  Three instructions where
+// the division takes ten; scales out of that range divide.
 struct Divisor {
   float scale, reciprocal;
-  bool plain;
-  __device__ __forceinline__ explicit Divisor(float s)
-      : scale(s), reciprocal(1.0f / s), plain(!(s >= 0x1p-100f && s <= 0x1p100f)) {}
+  __device__ __forceinline__ explicit Divisor(float s) : scale(s), reciprocal(1.0f / s) {}
+  __device__ __forceinline__ bool in_range() const { return scale >= 0x1p-100f && scale <= 0x1p100f; }
   __device__ __forceinline__ float operator()(float y) const {
-    if (plain) return y / scale;
     const float q = y * reciprocal;
     return __builtin_fmaf(__builtin_fmaf(-q, scale, y), reciprocal, q);
   }
@@ -75,28 +73,41 @@ __device__ __forceinline__ float scale_of(uint32_t amax_bits) {
 }
 
 template <int kFormat>
-__device__ __forceinline__ uint2 quantize8(const float (&y)[8], const Divisor& divide) {
+__device__ __forceinline__ uint2 codes8(const float (&q)[8]) {
   uint2 out;
   if constexpr (kFormat == kQuantInt8) {
+    // Added to 1.5 * 2^23 a quotient is rounded to a whole number, ties to even, whose two's complement is in the
+    // low byte; NaN gives some code, which its NaN scale makes NaN again.
     uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = __builtin_rintf(divide(y[i]));
-      // A NaN takes the lower bound: the code is a number, the scale is none.
-      b[i] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f))) & 0xffu;
-    }
-    out.x = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
-    out.y = b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24);
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(q[i] + 12582912.0f);
+    out.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u),
+                                  0x05040100u);
+    out.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[7], b[6], 0x0c0c0400u), __builtin_amdgcn_perm(b[5], b[4], 0x0c0c0400u),
+                                  0x05040100u);
   } else {
     int lo = 0, hi = 0;  // the conversion rounds to nearest even; quotients end at 448 by construction
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(divide(y[0]), divide(y[1]), lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(divide(y[2]), divide(y[3]), lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(divide(y[4]), divide(y[5]), hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(divide(y[6]), divide(y[7]), hi, true);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
     out.x = static_cast<uint32_t>(lo);
     out.y = static_cast<uint32_t>(hi);
   }
   return out;
+}
+
+template <int kFormat>
+__device__ __forceinline__ uint2 quantize8(const float (&y)[8], const Divisor& divide) {
+  float q[8];
+  if (__builtin_expect(divide.in_range(), 1)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = divide(y[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = y[i] / divide.scale;
+  }
+  return codes8<kFormat>(q);
 }
 
 __device__ __forceinline__ void unpack8(const vec16 v, float (&f)[8]) {
@@ -109,7 +120,7 @@ __device__ __forceinline__ void unpack8(const vec16 v, float (&f)[8]) {
 __device__ __forceinline__ vec16 pack8(const float (&f)[8]) {
   vec16 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) v[i] = to_bf16_pair(f[2 * i], f[2 * i + 1]);
   return v;
 }
 
@@ -136,10 +147,10 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
   for (int u = 0; u < kVecs; ++u) {
     const int v = t + u * kRowThreads;
     if (v < a.row_vecs) {
-      unpack8(x[v], y[u]);
+      unpack8(__builtin_nontemporal_load(x + v), y[u]);  // read once: not worth the cache it would take
       if (kNorm && residual != nullptr) {
         float r[8];
-        unpack8(residual[v], r);
+        unpack8(__builtin_nontemporal_load(residual + v), r);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[u][i] += r[i];
         if (a.residual_out != nullptr) a.residual_out[static_cast<size_t>(row) * a.row_vecs + v] = pack8(y[u]);
@@ -197,7 +208,8 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) m = umax(m, maxima[w]);
     }
-    const float scale = scale_of<kFormat>(m);
+    // One value for the whole row: in a scalar register the range test costs no vector instruction.
+    const float scale = wave_read(scale_of<kFormat>(m), 0);
     if (t == 0) *scales = scale;
     const Divisor divide(scale);
 #pragma unroll
@@ -246,7 +258,8 @@ __global__ __launch_bounds__(256) void ep_dequantize_rows_kernel(const Dequantiz
       }
       f[j] *= scale;
     }
-    a.out[i] = pack8(f);
+    if (a.stream_output) __builtin_nontemporal_store(pack8(f), a.out + i);
+    else a.out[i] = pack8(f);
   }
 }
 
@@ -258,7 +271,10 @@ hipError_t launch_quantize_as(const QuantizeArgs& a, hipStream_t stream) {
   const auto wide_rows = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.num_rows)), dim3(threads), 0, stream, a);
   };
-  if (a.row_vecs <= 64) wave_rows(&ep_quantize_rows_kernel<64, 1, kNorm, kFormat>);
+  // With fewer rows than compute units the latency of one row is the time: more threads to a row, fewer vectors each
+  // (16 rows of 7168 columns: 6.6 us with 256 threads of four vectors, 4.8 us with 1024 of one).
+  if (a.num_rows <= 256 && a.row_vecs > 512 && a.row_vecs <= 1024) wide_rows(&ep_quantize_rows_kernel<1024, 1, kNorm, kFormat>, 1024);
+  else if (a.row_vecs <= 64) wave_rows(&ep_quantize_rows_kernel<64, 1, kNorm, kFormat>);
   else if (a.row_vecs <= 128) wave_rows(&ep_quantize_rows_kernel<64, 2, kNorm, kFormat>);
   else if (a.row_vecs <= 256) wave_rows(&ep_quantize_rows_kernel<64, 4, kNorm, kFormat>);
   else if (a.row_vecs <= 512) wave_rows(&ep_quantize_rows_kernel<64, 8, kNorm, kFormat>);
@@ -279,8 +295,14 @@ hipError_t launch_quantize_rows(const QuantizeArgs& a, int format, hipStream_t s
   return norm ? launch_quantize_as<true, kQuantE4m3>(a, stream) : launch_quantize_as<false, kQuantE4m3>(a, stream);
 }
 
-hipError_t launch_dequantize_rows(const DequantizeArgs& a, int format, hipStream_t stream) {
-  if (a.num_rows == 0) return hipSuccess;
+hipError_t launch_dequantize_rows(const DequantizeArgs& args, int format, hipStream_t stream) {
+  if (args.num_rows == 0) return hipSuccess;
+  DequantizeArgs a = args;
+  // An output of a good part of the memory-side cache's size goes straight to HBM: what it would push out of that
+  // cache (the codes themselves, the norm's other outputs) is read again sooner than its first rows.  Quantising
+  // and reading back 65536 x 2048: 141 us with the store left to the caches, 124 us; norm and reading back 8192 x
+  // 7168: 103 and 99 us.
+  a.stream_output = static_cast<long long>(a.num_rows) * a.row_vecs * 16 >= (64ll << 20);
   const long long units = static_cast<long long>(a.num_rows) * a.row_vecs;
   const long long blocks = (units + 255) / 256;
   const dim3 grid(static_cast<unsigned>(blocks < 16384 ? blocks : 16384));

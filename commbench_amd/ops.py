@@ -515,13 +515,19 @@ def pull_indices(recv_src_map: torch.Tensor, tokens_per_source_rank: int,
 def _launch(device: torch.device, name: str, *args) -> None:
     """Calls an entry point on the current stream of the tensors' device, whichever device is current."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            code = fn(*args, torch.cuda.current_stream().cuda_stream)
+            code = fn(*args, _raw_stream(index))
     if code != 0:
         _lib.check(code, name)
+
+
+# The stream's handle without the Stream object around it (3 us of a call), where this build of torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _quant_format(quant: str, width: int):
