@@ -696,7 +696,7 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
 size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int intermediate) {
   if (!few_tokens_shape_ok(num_tokens, num_topk) || intermediate <= 0 || intermediate % 16 != 0 || intermediate > 65536)
     return 0;
-  return static_cast<size_t>(num_tokens) * num_topk * intermediate * 2;
+  return static_cast<size_t>(num_tokens) * num_topk * intermediate * 4;
 }
 
 int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* topk_weights, const void* w13,

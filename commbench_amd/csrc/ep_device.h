@@ -264,7 +264,7 @@ struct FewTokensArgs {
   const float* w2_scales;     // [num_experts, hidden]
   const uint16_t* bias_0;
   const uint16_t* bias_1;
-  uint16_t* act;  // bf16 [num_tokens * num_topk, intermediate]
+  uint16_t* act;  // bf16 [2, num_tokens * num_topk, intermediate]: two terms of every value
   uint16_t* combined_x;
   int num_tokens;
   int num_topk;

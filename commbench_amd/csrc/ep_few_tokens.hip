@@ -5,7 +5,8 @@
 // experts' weights once; moving rows to the experts and back would only add launches.  Weights are
 // bf16, or int8 with a scale for each output channel (widened to bf16 in registers, exactly), products
 // run on the matrix units with the weights as the 16-row operand and up to 16 of an expert's routes as
-// the columns, sums are fp32.  act is rounded to bf16, the type the many-token path hands on there too.
+// the columns, sums are fp32.  act is kept as the sum of two bf16 values (16 bits: one alone would be as large an
+// error as the rounding of the result), which the second product takes as two columns.
 // A sum never depends on the order in which waves finish: each (route, output) has one writer, and the
 // slots of a token are added in ascending order at the end.
 #include <atomic>
@@ -58,7 +59,6 @@ struct Chunk {
   static constexpr int kElements = 4 * kLane;     // of k
   static constexpr int kVectors = kInt8 ? 2 : 1;  // 16-byte bf16 loads of a column for a load of weights
   static constexpr int kAll = 2 * kVectors;       // and for a lane's whole chunk
-  static constexpr int kFoldColumns = 16 / kAll;  // columns of a folded load
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int bytes) {
@@ -146,22 +146,27 @@ struct Meeting {
 // used is filled with the one kDepth further on, also across the end of an item, whose number of chunks
 // is rounded up to a multiple of kDepth (the excess loads nothing).
 //
-// Folded (passes of no more than kFoldColumns columns): most of a column load's 16 columns would be empty, so one
-// load fetches all of a lane's kAll vectors for kFoldColumns columns, vector v in columns v * kFoldColumns and
-// on.  Product v then has its sums in those columns of its own accumulator, and the accumulators are put
-// together when the item ends.
-template <bool kInt8, int kMatrices, int kColumns, int kDepth, bool kFold>
+// The 16 columns of a block are kFold vectors times kParts values (bf16 terms of one number) times kRoutes routes.
+// kFold > 1 serves experts with few routes, where most columns would be empty: one load then fetches kFold of a
+// lane's kAll vectors, vector v in the columns of fold v % kFold.  Product v has its sums in those columns of
+// accumulator v % kFold; folds and parts are added up when the item ends.
+template <bool kInt8, int kMatrices, int kBlocks, int kDepth, int kFold, int kParts>
 struct Stream {
   using C = Chunk<kInt8>;
-  static_assert(!kFold || kColumns == 1, "only a single block of columns folds");
-  static constexpr int kSums = kFold ? C::kAll : kColumns;
-  vec16 w[kDepth][2][kMatrices], x[kDepth][kFold ? 1 : 2][kColumns][kFold ? 1 : C::kVectors];
+  static constexpr int kRoutes = 16 / (kFold * kParts);
+  static constexpr int kLoads = C::kAll / kFold;
+  static_assert(kLoads * kFold == C::kAll && (kFold == 1 || kBlocks == 1), "a fold fits a lane's vectors; blocks do not fold");
+  vec16 w[kDepth][2][kMatrices], x[kDepth][kBlocks][kLoads];
 
   // Where the loads stand: an item's weights and columns, and the next chunk.
   const unsigned char* rows[kMatrices];
   int row_bytes;  // of 16 rows
-  int w_lane, x_at[kColumns], k, k_end;
+  int w_lane, x_at[kBlocks], k, k_end;
 
+  // The lane's column: route, part and fold.
+  static __device__ __forceinline__ int lane_route() { return lane_id() & (kRoutes - 1); }
+  static __device__ __forceinline__ int lane_part() { return (lane_id() / kRoutes) & (kParts - 1); }
+  static __device__ __forceinline__ int lane_fold() { return (lane_id() & 15) / (16 / kFold); }
 
   __device__ __forceinline__ void load(int slot, __amdgpu_buffer_rsrc_t vectors) {
 #pragma unroll
@@ -172,26 +177,17 @@ struct Stream {
       for (int m = 0; m < kMatrices; ++m)
         w[slot][h][m] = __builtin_amdgcn_raw_buffer_load_b128(rows_of(rows[m], row_bytes), at, 0, 0);
     }
-    if constexpr (kFold) {  // x_at includes the lane's vector
-      const int v = (lane_id() & 15) / C::kFoldColumns;
-      x[slot][0][0][0] = __builtin_amdgcn_raw_buffer_load_b128(
-          vectors, k + v / C::kVectors * C::kPiece < k_end ? x_at[0] + k * 2 : kOutside, 0, 0);
-    } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bool inside = k + h * C::kPiece < k_end;
+    for (int l = 0; l < kLoads; ++l) {
+      const int v = l * kFold + (kFold > 1 ? lane_fold() : 0);
+      const bool inside = k + v / C::kVectors * C::kPiece < k_end;
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-          const int from = inside ? x_at[c] + k * 2 : kOutside;
-#pragma unroll
-          for (int v = 0; v < C::kVectors; ++v)
-            x[slot][h][c][v] = __builtin_amdgcn_raw_buffer_load_b128(vectors, from + 16 * (h * C::kVectors + v), 0, 0);
-        }
-      }
+      for (int c = 0; c < kBlocks; ++c)
+        x[slot][c][l] = __builtin_amdgcn_raw_buffer_load_b128(vectors, inside ? x_at[c] + k * 2 + v * 16 : kOutside, 0, 0);
     }
     k += C::kElements;
   }
-  __device__ __forceinline__ void use(int slot, float4v (&acc)[kMatrices][kSums]) const {
+  __device__ __forceinline__ void use(int slot, float4v (&acc)[kMatrices][kBlocks][kFold]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -205,14 +201,27 @@ struct Stream {
           rows16[0] = as_bf16(packed);
         }
 #pragma unroll
-        for (int v = 0; v < C::kVectors; ++v)
+        for (int i = 0; i < C::kVectors; ++i) {
+          const int v = h * C::kVectors + i;
 #pragma unroll
-          for (int c = 0; c < kColumns; ++c) {
-            const int sum = kFold ? h * C::kVectors + v : c;
-            const bf16x8 columns16 = as_bf16(kFold ? x[slot][0][0][0] : x[slot][kFold ? 0 : h][c][kFold ? 0 : v]);
-            acc[m][sum] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows16[v], columns16, acc[m][sum], 0, 0, 0);
-          }
+          for (int c = 0; c < kBlocks; ++c)
+            acc[m][c][v % kFold] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows16[i], as_bf16(x[slot][c][v / kFold]),
+                                                                           acc[m][c][v % kFold], 0, 0, 0);
+        }
       }
+  }
+  // The sums of a block, complete in the lanes of fold 0 and part 0.
+  static __device__ __forceinline__ float4v total(const float4v (&acc)[kFold]) {
+    float4v sum = acc[0];
+    if constexpr (kFold * kParts > 1) {
+      const int base = (lane_id() & 48) + lane_route();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int other = 1; other < kFold * kParts; ++other)
+          sum[i] += __shfl(acc[other / kParts][i], base + other * kRoutes);
+    }
+    return sum;
   }
 };
 
@@ -247,7 +256,7 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
   const int k_stop = share_end < H ? share_end : H;
 
   const __amdgpu_buffer_rsrc_t vectors = rows_of(a.x, a.num_tokens * H * 2);
-  Stream<kInt8, 2, kColumns, kDepth, false> s;
+  Stream<kInt8, 2, kColumns, kDepth, 1, 1> s;
   s.row_bytes = 16 * H * C::kBytes;
   s.w_lane = (lane & 15) * H * C::kBytes;
   int column[kColumns], next_route[kColumns], route[kColumns];
@@ -279,9 +288,9 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
   for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
 
   for (int item = from; item < to; ++item) {
-    float4v acc[2][kColumns];
+    float4v acc[2][kColumns][1];
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) acc[0][c] = acc[1][c] = float4v{0, 0, 0, 0};
+    for (int c = 0; c < kColumns; ++c) acc[0][c][0] = acc[1][c][0] = float4v{0, 0, 0, 0};
     for (int round = 0; round < rounds; ++round) {
       if (round == rounds - 1) {
         ++ahead;
@@ -303,8 +312,8 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
       float(&sums)[kFirstWaves][2][4][kWave] = partial[(item * kColumns + c) & 1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sums[wave][0][i][lane] = acc[0][c][i];
-        sums[wave][1][i][lane] = acc[1][c][i];
+        sums[wave][0][i][lane] = acc[0][c][0][i];
+        sums[wave][1][i][lane] = acc[1][c][0][i];
       }
       wait_lds_and_meet();
       const int column_route = __shfl(route[c], j);
@@ -320,8 +329,13 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
           g *= scales[0];
           u *= scales[I];
         }
-        a.act[static_cast<size_t>(column_route) * I + i0 + n] =
-            static_cast<uint16_t>(f32_to_bf16_bits(g / (1.0f + __expf(-g)) * u));
+        const float act = g / (1.0f + __expf(-g)) * u;
+        const uint32_t high = f32_to_bf16_bits(act);
+        uint16_t* out = a.act + static_cast<size_t>(column_route) * I + i0 + n;
+        out[0] = static_cast<uint16_t>(high);
+        // The rest of an infinity is none.
+        const float rest = act - bf16_lo(high);
+        out[static_cast<size_t>(routes) * I] = __builtin_isfinite(act) ? static_cast<uint16_t>(f32_to_bf16_bits(rest)) : 0;
       }
     }
 #pragma unroll
@@ -331,11 +345,12 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
 
 // Down.  Workgroup h: 16 columns of the output for every token.  Items are the entries (with fewer of them than
 // waves, shares of their k); wave w takes items w, w + 8, ...  y[split][route][16] collects the products.
-template <bool kInt8, int kColumns, int kDepth, bool kFold>
+template <bool kInt8, int kBlocks, int kDepth, int kFold>
 __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(const FewTokensArgs a, const int splits) {
   using C = Chunk<kInt8>;
   extern __shared__ __align__(16) unsigned char shared[];
-  constexpr int kPass = kFold ? C::kFoldColumns : 16 * kColumns;
+  using S = Stream<kInt8, 1, kBlocks, kDepth, kFold, 2>;
+  constexpr int kPass = S::kRoutes * kBlocks;
   __shared__ uint16_t lists[kSecondWaves][kPass];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int routes = a.num_tokens * a.num_topk;
@@ -351,15 +366,14 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
   const int rounds = (share + kDepth - 1) / kDepth;
   const int k_lane = (lane >> 4) * C::kLane;
 
-  const __amdgpu_buffer_rsrc_t vectors = rows_of(a.act, routes * I * 2);
-  Stream<kInt8, 1, kColumns, kDepth, kFold> s;
-  constexpr int kSums = Stream<kInt8, 1, kColumns, kDepth, kFold>::kSums;
+  const __amdgpu_buffer_rsrc_t vectors = rows_of(a.act, routes * I * 4);
+  S s;
   s.row_bytes = 16 * I * C::kBytes;
   s.w_lane = (lane & 15) * I * C::kBytes;
-  int column[kColumns], next_route[kColumns], route[kColumns];
+  int column[kBlocks], next_route[kBlocks], route[kBlocks];
 #pragma unroll
-  for (int c = 0; c < kColumns; ++c) column[c] = kFold ? lane & (C::kFoldColumns - 1) : c * 16 + (lane & 15);
-  const int vector_at = kFold ? (lane & 15) / C::kFoldColumns * 16 : 0;
+  for (int c = 0; c < kBlocks; ++c) column[c] = c * S::kRoutes + S::lane_route();
+  const int part_at = S::lane_part() * routes * I * 2;
   int ahead = wave;
   const auto begin_item = [&]() {
     if (ahead >= items) {
@@ -367,9 +381,9 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
       return;
     }
     const int entry = ahead / splits, split = ahead - entry * splits;
-    meeting.template columns<kColumns>(entry, routes, lists[wave], column, next_route);
+    meeting.template columns<kBlocks>(entry, routes, lists[wave], column, next_route);
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] * I * 2 + vector_at : kOutside;
+    for (int c = 0; c < kBlocks; ++c) s.x_at[c] = next_route[c] >= 0 ? next_route[c] * I * 2 + part_at : kOutside;
     s.rows[0] = a.w2 + (static_cast<size_t>(meeting.expert(entry)) * H + h0) * I * C::kBytes;
     const int end = share * (split + 1) * C::kElements;
     s.k = share * split * C::kElements + k_lane;
@@ -380,12 +394,14 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) s.load(d, vectors);
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
+    for (int c = 0; c < kBlocks; ++c) route[c] = next_route[c];
   }
   for (int item = wave; item < items; item += kSecondWaves) {
-    float4v acc[1][kSums];
+    float4v acc[1][kBlocks][kFold];
 #pragma unroll
-    for (int c = 0; c < kSums; ++c) acc[0][c] = float4v{0, 0, 0, 0};
+    for (int c = 0; c < kBlocks; ++c)
+#pragma unroll
+      for (int f = 0; f < kFold; ++f) acc[0][c][f] = float4v{0, 0, 0, 0};
     for (int round = 0; round < rounds; ++round) {
       if (round == rounds - 1) {
         ahead += kSecondWaves;
@@ -398,18 +414,6 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    float4v sum[kColumns];
-    if constexpr (kFold) {
-      sum[0] = acc[0][0];
-#pragma unroll
-      for (int v = 1; v < kSums; ++v)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[0][i] += __shfl(acc[0][v][i], (lane & 48) + v * C::kFoldColumns + column[0]);
-      if ((lane & 15) >= C::kFoldColumns) route[0] = -1;  // lanes that held other vectors of the same columns
-    } else {
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c) sum[c] = acc[0][c];
-    }
     const int entry = item / splits, split = item - entry * splits;
     const int n = (lane >> 4) * 4;
     float scales[4] = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -418,9 +422,10 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
       scales[0] = of.x, scales[1] = of.y, scales[2] = of.z, scales[3] = of.w;
     }
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) {
-      if (route[c] >= 0) {
-        const float4 out = {sum[c][0] * scales[0], sum[c][1] * scales[1], sum[c][2] * scales[2], sum[c][3] * scales[3]};
+    for (int c = 0; c < kBlocks; ++c) {
+      const float4v sum = S::total(acc[0][c]);
+      if (route[c] >= 0 && (lane & 15) < S::kRoutes) {
+        const float4 out = {sum[0] * scales[0], sum[1] * scales[1], sum[2] * scales[2], sum[3] * scales[3]};
         *reinterpret_cast<float4*>(y + (split * routes + route[c]) * 16 + n) = out;
       }
       route[c] = next_route[c];
@@ -459,7 +464,7 @@ hipError_t launch_gate_up(const FewTokensArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <bool kInt8, int kColumns, int kDepth, bool kFold>
+template <bool kInt8, int kBlocks, int kDepth, int kFold>
 hipError_t launch_down(const FewTokensArgs& a, hipStream_t stream) {
   const int routes = a.num_tokens * a.num_topk;
   const int splits = routes >= kSecondWaves ? 1 : kSecondWaves / routes;
@@ -475,13 +480,13 @@ hipError_t launch_down(const FewTokensArgs& a, hipStream_t stream) {
     static std::atomic<int> lds_limit_raised[kMaxDevices];
     if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
     if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kColumns, kDepth, kFold>),
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kBlocks, kDepth, kFold>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
       if (e != hipSuccess) return e;
       lds_limit_raised[ordinal].store(1, std::memory_order_release);
     }
   }
-  hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8, kColumns, kDepth, kFold>), dim3(static_cast<unsigned>(a.hidden / 16)),
+  hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8, kBlocks, kDepth, kFold>), dim3(static_cast<unsigned>(a.hidden / 16)),
                      dim3(kSecondThreads), lds, stream, a, splits);
   return hipGetLastError();
 }
@@ -493,9 +498,9 @@ hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
   const bool many = routes > 8 * a.num_experts;
   const hipError_t e = many ? launch_gate_up<kInt8, 4, 1>(a, stream) : launch_gate_up<kInt8, 1, 2>(a, stream);
   if (e != hipSuccess) return e;
-  if (many) return launch_down<kInt8, 4, kInt8 ? 1 : 2, false>(a, stream);
-  if (routes > (kInt8 ? 2 : 4) * a.num_experts) return launch_down<kInt8, 1, 4, false>(a, stream);
-  return launch_down<kInt8, 1, 4, true>(a, stream);
+  if (many) return launch_down<kInt8, 4, 1, 1>(a, stream);
+  if (routes > 2 * a.num_experts) return launch_down<kInt8, 1, 4, 1>(a, stream);
+  return launch_down<kInt8, 1, 4, 2>(a, stream);
 }
 
 }  // namespace

@@ -460,7 +460,7 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
  *   workspace    mi_ep_moe_few_tokens_workspace_bytes bytes, 16-byte aligned, no initialisation; calls that
  *                share one must not overlap in time
  * Sums are fp32 in an order that depends on the shapes alone; the activation between the two products is
- * rounded to bf16.  num_tokens * num_topk <= MI_EP_FEW_MAX_ROUTES; hidden % 16 == 0, intermediate % 16 == 0, both
+ * carried in 16 bits of mantissa.  num_tokens * num_topk <= MI_EP_FEW_MAX_ROUTES; hidden % 16 == 0, intermediate % 16 == 0, both
  * at most 65536; x, w13, w2, biases and combined_x 16-byte aligned.
  */
 #define MI_EP_FEW_MAX_ROUTES 1024

@@ -51,7 +51,7 @@ def few_tokens64(x, ids, gates, w13, w2, s13, s2, biases=()):
     """(out, bound) of the expert layer in 64 bits.  x, w13, w2 hold the operands' values in float64 (int8
     codes for quantised weights), the scales float64 or None.  The bound counts: n products summed in
     fp32 (n + 8 roundings of at most a whole step, 2 U, of the sum of magnitudes), silu * up, the
-    activation's rounding to bf16, the second sum, the weighted sum over the slots, and the last rounding."""
+    activation's rounding to two bf16 terms, the second sum, the weighted sum over the slots, and the last rounding."""
     T, K = ids.shape
     E, H, I = w2.shape
     out = np.zeros((T, H))
@@ -69,7 +69,7 @@ def few_tokens64(x, ids, gates, w13, w2, s13, s2, biases=()):
             c_err = (H + 8) * 2 * U * (np.abs(a) @ np.abs(x[t])) * np.abs(one)
             act = silu64(c[:I]) * c[I:]
             act_err = silu_mul_bound(c[:I], c[I:], c_err[:I], c_err[I:])
-            act_err = act_err + BF16 * (np.abs(act) + act_err) + 2.0 ** -133
+            act_err = act_err + BF16 ** 2 * (np.abs(act) + act_err) + 2.0 ** -133   # two bf16 terms: half a step of half a step
             y = (b @ act) * two
             y_err = (np.abs(b) @ act_err + (I + 8) * 2 * U * (np.abs(b) @ (np.abs(act) + act_err))) * np.abs(two)
             w = float(gates[t, k]) if gates is not None else 1.0

@@ -156,10 +156,10 @@ def test_captured_graphs_replay_with_new_inputs_next_to_each_other():
 
 def test_workspace_size_is_checked_and_no_tokens_is_no_work():
     lib = _lib.load()
-    assert lib.mi_ep_moe_few_tokens_workspace_bytes(128, 8, 2048) == 128 * 8 * 2048 * 2
+    assert lib.mi_ep_moe_few_tokens_workspace_bytes(128, 8, 2048) == 128 * 8 * 2048 * 4
     g = on_gpu(problem(25, 2, 4, 2, 64, 32, False))
     out = torch.full((2, 64), 5.0, dtype=torch.bfloat16, device=xu.DEV)
-    work = torch.empty(2 * 2 * 32 * 2, dtype=torch.uint8, device=xu.DEV)
+    work = torch.empty(2 * 2 * 32 * 4, dtype=torch.uint8, device=xu.DEV)
     args = lambda nbytes: (g["x"].data_ptr(), g["ids"].data_ptr(), g["gates"].data_ptr(), g["w13"].data_ptr(), None,
                            g["w2"].data_ptr(), None, None, None, 2, 2, 4, 64, 32, out.data_ptr(), work.data_ptr(), nbytes,
                            torch.cuda.current_stream().cuda_stream)
