@@ -45,7 +45,7 @@ inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7
 // Rows of the 8-bit formats; the scales' strides count floats.
 inline bool quantized_shape_ok(int num_rows, int hidden, int format, long long scales_row_stride,
                                long long scales_hidden_stride) {
-  if (num_rows < 0 || hidden <= 0 || hidden % 8 != 0 || hidden > MI_EP_QUANT_MAX_HIDDEN) return false;
+  if (num_rows < 0 || num_rows >= (1 << 30) || hidden <= 0 || hidden % 8 != 0 || hidden > MI_EP_QUANT_MAX_HIDDEN) return false;
   if (format != MI_EP_QUANT_INT8_ROW && format != MI_EP_QUANT_E4M3_BLOCK) return false;
   if (format == MI_EP_QUANT_E4M3_BLOCK && hidden % MI_EP_QUANT_BLOCK != 0) return false;
   return scales_row_stride >= 0 && (format == MI_EP_QUANT_INT8_ROW || scales_hidden_stride >= 0);
@@ -667,10 +667,12 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
                               int in_features, void* out, int flags, void* stream) {
   const bool silu_mul = (flags & MI_EP_MATMUL_SILU_MUL) != 0;
   if ((flags & ~MI_EP_MATMUL_SILU_MUL) != 0) return MI_EP_EINVAL;
-  if (num_rows < 0 || num_rows >= (1 << 30) || num_experts <= 0 || num_experts > MI_EP_MAX_EXPERTS) return MI_EP_EINVAL;
+  if (num_rows < 0 || num_rows >= (1 << 28) || num_experts <= 0 || num_experts > MI_EP_MAX_EXPERTS) return MI_EP_EINVAL;
   // |a * b| <= 2^14: 2^17 of them are the most whose sum is sure to fit 32 bits.
   if (in_features <= 0 || in_features % 16 != 0 || in_features >= (1 << 17)) return MI_EP_EINVAL;
   if (out_features <= 0 || out_features % (silu_mul ? 16 : 8) != 0 || out_features > (1 << 20)) return MI_EP_EINVAL;
+  // Tiles of the product are counted in int.
+  if ((num_rows / 256 + num_experts) * (out_features / 128 + 1LL) >= (1LL << 31)) return MI_EP_EINVAL;
   if (a_scales_row_stride < 0 || a_scales_row_stride > (1 << 20)) return MI_EP_EINVAL;  // a tile's scales lie within 2^30 bytes
   if (expert_offsets == nullptr && (num_experts != 1 || num_tokens_per_expert != nullptr)) return MI_EP_EINVAL;
   if (!aligned16(a) || !aligned16(b) || !aligned16(out)) return MI_EP_EINVAL;

@@ -219,6 +219,7 @@ struct QuantizeArgs {
   long long scales_row_stride, scales_hidden_stride;  // in floats
   int num_rows;
   int row_vecs;
+  int first_row;  // of the launch; set by the launcher
   float eps;
 };
 hipError_t launch_quantize_rows(const QuantizeArgs& a, int format, hipStream_t stream);

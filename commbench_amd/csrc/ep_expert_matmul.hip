@@ -514,7 +514,11 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
 
   // Workgroups go to the eight dies in turn; each die takes one contiguous run of the tiles, so that the rows
   // and weights its compute units share come from its own L2.
-  const int total = __builtin_amdgcn_readfirstlane(tiles_before[kBigThreads]) * column_tiles;
+  // Segments that do not overlap make no more tiles than this; what overlapping ones (tables of a layout that gave
+  // up) would make beyond is not computed.
+  const int most = a.num_rows / (kMaxBlocks * kBlockRows) + a.num_experts;
+  const int made = __builtin_amdgcn_readfirstlane(tiles_before[kBigThreads]);
+  const int total = (made < most ? made : most) * column_tiles;
   const int dies = gridDim.x % 8 == 0 ? 8 : 1;
   const int per_die = (total + dies - 1) / dies;
   const int die = static_cast<int>(blockIdx.x) % dies;

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
   __shared__ uint32_t maxima[kWaves];
   const int t = kRows == 1 ? static_cast<int>(threadIdx.x) : lane_id();
   const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const int row = static_cast<int>(blockIdx.x) * kRows + (kRows == 1 ? 0 : wave);
+  const int row = a.first_row + static_cast<int>(blockIdx.x) * kRows + (kRows == 1 ? 0 : wave);
   int rows = a.num_rows;
   if (a.row_limit != nullptr && *a.row_limit < rows) rows = *a.row_limit;
   if (row >= rows) return;  // the same for every thread that meets the barriers below
@@ -264,13 +264,21 @@ __global__ __launch_bounds__(256) void ep_dequantize_rows_kernel(const Dequantiz
 }
 
 template <bool kNorm, int kFormat>
-hipError_t launch_quantize_as(const QuantizeArgs& a, hipStream_t stream) {
-  const auto wave_rows = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.num_rows + 3) / 4)), dim3(4 * kWave), 0, stream, a);
+hipError_t launch_quantize_as(const QuantizeArgs& args, hipStream_t stream) {
+  // A launch has fewer than 2^32 threads: very many rows take several.
+  const auto in_pieces = [&](auto kernel, int rows_at_once, int threads, int rows_per_group) {
+    QuantizeArgs a = args;
+    for (long long first = 0; first < args.num_rows; first += rows_at_once) {
+      const long long left = args.num_rows - first;
+      const long long rows = left < rows_at_once ? left : rows_at_once;
+      a.first_row = static_cast<int>(first);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((rows + rows_per_group - 1) / rows_per_group)), dim3(threads), 0,
+                         stream, a);
+    }
   };
-  const auto wide_rows = [&](auto kernel, int threads) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.num_rows)), dim3(threads), 0, stream, a);
-  };
+  const auto wave_rows = [&](auto kernel) { in_pieces(kernel, 1 << 25, 4 * kWave, 4); };
+  const auto wide_rows = [&](auto kernel, int threads) { in_pieces(kernel, 1 << 21, threads, 1); };
+  const QuantizeArgs& a = args;
   // With fewer rows than compute units the latency of one row is the time: more threads to a row, fewer vectors each
   // (16 rows of 7168 columns: 6.6 us with 256 threads of four vectors, 4.8 us with 1024 of one).
   if (a.num_rows <= 256 && a.row_vecs > 512 && a.row_vecs <= 1024) wide_rows(&ep_quantize_rows_kernel<1024, 1, kNorm, kFormat>, 1024);

@@ -289,6 +289,8 @@ class Buffer:
         _require(w13.dim() == 3 and w2.dim() == 3 and w13.shape[0] == self.num_experts and w2.shape[0] == self.num_experts
                  and w13.shape[1] == 2 * w2.shape[2] and w2.shape[1] == w13.shape[2] == q.shape[1],
                  "w13 must be [experts, 2 * intermediate, hidden] and w2 [experts, hidden, intermediate]")
+        if q.shape[0] == 0:
+            return torch.empty((0, q.shape[1]), dtype=torch.bfloat16, device=q.device)
         recv, recv_scales, _, h = self.dispatch(q, scales, topk_idx, topk_weights, expert_alignment)
         act = grouped_matmul_int8(recv, recv_scales, w13, w13_scales, h.expert_offsets, h.num_tokens_per_expert, "silu_mul")
         act_q, act_scales = quantize_rows(act, row_limit=h.expert_offsets[-1:])
@@ -678,7 +680,7 @@ def grouped_matmul_int8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor
                      and num_tokens_per_expert.device == dev and tuple(num_tokens_per_expert.shape) == (experts,)),
                  "num_tokens_per_expert must be contiguous int32 [experts]")
     out = torch.empty((rows, n // 2 if activation else n), dtype=torch.bfloat16, device=dev)
-    _launch(dev, "mi_ep_grouped_matmul_int8", a.data_ptr(), a_scales.data_ptr(), a_scales.stride(0), b.data_ptr(),
+    _launch(dev, "mi_ep_grouped_matmul_int8", a.data_ptr(), a_scales.data_ptr(), a_scales.stride(0) if rows > 1 else 1, b.data_ptr(),
             b_scales.data_ptr(), _ptr(expert_offsets), _ptr(num_tokens_per_expert), rows, experts, n, k, out.data_ptr(),
             SILU_MUL if activation else 0)
     return out

@@ -405,7 +405,9 @@ int mi_ep_combine(const void* y, int num_rows, const int* slot_map, const float*
  *                row stride of hidden); needs residual
  *   normed       bf16 [num_rows, hidden] or NULL: y rounded once (for a router or a bf16 branch)
  * A row (block) that holds an infinity or a NaN gets a NaN scale and reads back as NaN throughout.
- * hidden % 8 == 0, hidden <= 32768; bf16 pointers 16-byte aligned.  Outputs must not overlap inputs otherwise.
+ * (as does a row of zeros under epsilon 0).
+ * hidden % 8 == 0, hidden <= 32768, num_rows < 2^30; bf16 pointers 16-byte aligned.  Outputs must not overlap
+ * inputs otherwise.
  * mi_ep_dequantize_rows reads them back: out = bf16(q * scale).
  */
 #define MI_EP_QUANT_INT8_ROW 0
@@ -437,8 +439,9 @@ int mi_ep_dequantize_rows(const void* q, const float* scales, long long scales_r
  *                expert_offsets[e] .. + num_tokens_per_expert[e] (to expert_offsets[e + 1] when the counts are
  *                NULL: pad rows are computed too).  Both NULL with num_experts == 1: one expert owns all rows.
  *   out          bf16 [num_rows, out_features or I]; rows that belong to no expert are left as they were
- * in_features % 16 == 0 and below 131072, out_features % 8 == 0 (% 16 with SILU_MUL), num_experts <= 1024; a,
- * b, out 16-byte aligned.  num_rows is the capacity: segments are clamped to it.
+ * in_features % 16 == 0 and below 131072, out_features % 8 == 0 (% 16 with SILU_MUL) and at most 2^20,
+ * num_experts <= 1024, num_rows < 2^28, a_scales_row_stride <= 2^20; a, b, out 16-byte aligned.  num_rows is
+ * the capacity: segments are clamped to it.
  */
 #define MI_EP_MATMUL_SILU_MUL 1
 int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_scales_row_stride, const void* b,

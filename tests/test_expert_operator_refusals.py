@@ -20,7 +20,7 @@ def norm(x=A, xs=64, r=None, rs=64, w=A, eps=EPS, rows=4, h=64, fmt=0, q=A, s=A,
 
 
 @pytest.mark.parametrize("bad", [
-    dict(x=None), dict(w=None), dict(q=None), dict(s=None), dict(rows=-1), dict(h=0), dict(h=12), dict(h=32776, xs=32776),
+    dict(x=None), dict(w=None), dict(q=None), dict(s=None), dict(rows=-1), dict(rows=1 << 30), dict(h=0), dict(h=12), dict(h=32776, xs=32776),
     dict(fmt=2), dict(fmt=-1), dict(fmt=1, h=64), dict(xs=56), dict(xs=68), dict(r=A, rs=60), dict(x=A + 8), dict(w=A + 2),
     dict(q=A + 4), dict(r=A + 8), dict(ro=A), dict(r=A, ro=A + 8), dict(n=A + 8), dict(eps=0x7f800000), dict(eps=0x7fc00000),
     dict(eps=0xbf800000), dict(srs=0), dict(srs=-1), dict(fmt=1, h=256, xs=256, srs=1, shs=1), dict(fmt=1, h=256, xs=256, shs=0),
@@ -56,7 +56,7 @@ def test_product_refuses():
     def matmul(a=A, sa=A, sas=1, b=A, sb=A, off=A, cnt=A, rows=4, e=2, n=64, k=64, out=A, flags=0):
         return lib().mi_ep_grouped_matmul_int8(a, sa, sas, b, sb, off, cnt, rows, e, n, k, out, flags, None)
     for bad in (dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(out=None), dict(off=None, cnt=None),
-                dict(off=None, e=1), dict(rows=-1), dict(rows=1 << 30), dict(e=0), dict(e=1025), dict(n=0), dict(n=12), dict(n=24, flags=1),
+                dict(off=None, e=1), dict(rows=-1), dict(rows=1 << 28), dict(rows=(1 << 28) - 1, n=1 << 20), dict(sas=(1 << 20) + 1), dict(e=0), dict(e=1025), dict(n=0), dict(n=12), dict(n=24, flags=1),
                 dict(k=0), dict(k=24), dict(k=131072), dict(flags=2), dict(sas=-1), dict(a=A + 8), dict(b=A + 1), dict(out=A + 8)):
         assert matmul(**bad) == EINVAL, bad
 

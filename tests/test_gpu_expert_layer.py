@@ -132,3 +132,16 @@ def test_layer_captured_whole_and_replayed():
         torch.cuda.synchronize()
         assert torch.equal(held, eager)
     buf.status()
+
+
+def test_layer_of_no_tokens_and_of_masked_ones():
+    v = layer_inputs(11, 4, 8, 2, 256, 128, 0.0)
+    buf = ops.Buffer(4, 2, 8, 2, device=xu.DEV)
+    for align in (1, 16):
+        q, s = ops.quantize_rows(v["x"])
+        none = buf.moe_int8(q[:0], s[:0], v["ids"][:0], v["gates"][:0], v["w13"], v["s13"], v["w2"], v["s2"], expert_alignment=align)
+        assert none.shape == (0, 256)
+        masked = buf.moe_int8(q, s, torch.full_like(v["ids"], -1), v["gates"], v["w13"], v["s13"], v["w2"], v["s2"],
+                              bias=v["r"][:4].contiguous(), expert_alignment=align)
+        assert torch.equal(masked, v["r"][:4])
+    buf.status()

@@ -82,6 +82,67 @@ def test_product_against_integers(counts, n, k, silu):
     xu.check_within(xu.f64(out), want, bound)
 
 
+# 32 experts by four or more column tiles: enough for the large tiles.  Empty, single and full rows around their 32-,
+# 64- and 256-row edges; long segments in several tiles.
+LARGE = [1, 0, 31, 32, 33, 63, 64, 65, 0, 127, 128, 129, 191, 193, 255, 256, 257, 300, 0, 321, 385, 511, 512, 513, 700, 2, 5, 17,
+         0, 40, 90, 1]
+
+
+@pytest.mark.parametrize("k", [16, 48, 64, 80, 128, 144, 192, 208, 256, 320, 336, 1040])
+@pytest.mark.parametrize("n,silu", [(776, False), (1024, False), (1104, True)])
+def test_large_tiles_against_integers(n, k, silu):
+    """One to many steps over k, whole and partial ones, ragged last columns."""
+    print(f"large tiles out {n} in {k} silu {silu}", flush=True)
+    p = problem(n + k, LARGE, n, k, extra_rows=70)
+    want, bound, mine = reference(p, silu)
+    p["sa"][~mine] = np.nan
+    out = run_raw(p, silu)
+    xu.check_within(xu.f64(out)[mine], want[mine], bound[mine])
+    assert bool((out.cpu()[torch.from_numpy(~mine)] == -77.0).all())
+    assert torch.equal(run_raw(p, silu), out)                         # and the same again, to the bit
+
+
+@pytest.mark.parametrize("align", [16, 128])
+def test_large_tiles_with_pads_strided_scales_and_without_counts(align):
+    p = problem(77, LARGE, 768, 272, align)
+    want, bound, mine = reference(p, False)
+    p["sa"] = np.where(mine, p["sa"], np.nan).astype(np.float32)
+    out = run_raw(p, False)
+    xu.check_within(xu.f64(out)[mine], want[mine], bound[mine])
+    assert bool((out.cpu()[torch.from_numpy(~mine)] == -77.0).all())
+    a, b, sb, off, counts = (xu.to_gpu(p[key]) for key in ("a", "b", "sb", "off", "counts"))
+    wide = torch.full((p["a"].shape[0], 7), float("nan"), device=xu.DEV)
+    wide[:, 3] = xu.to_gpu(p["sa"])
+    got = ops.grouped_matmul_int8(a, wide[:, 3:4], b, sb, off, counts)
+    rows = torch.from_numpy(mine).to(xu.DEV)
+    assert torch.equal(got[rows], out[rows])
+    p["sa"] = np.nan_to_num(p["sa"], nan=0.5)
+    p["counts"] = np.diff(p["off"]).astype(np.int32)
+    want, bound, mine = reference(p, False)
+    xu.check_within(xu.f64(run_raw(p, False, use_counts=False))[mine], want[mine], bound[mine])
+
+
+def test_large_tiles_of_many_experts_and_of_one():
+    rng = np.random.default_rng(3)
+    for counts, n, k in ((rng.integers(0, 40, 600).tolist(), 512, 64), (rng.integers(5, 30, 1024).tolist(), 264, 48), ([8200], 776, 96)):
+        p = problem(len(counts), counts, n, k)
+        want, bound, _ = reference(p, False)
+        xu.check_within(xu.f64(run_raw(p, False)), want, bound)
+
+
+def test_large_tiles_on_tables_of_a_layout_that_gave_up():
+    """Overlapping, negative and out-of-range segments: in bounds, and an end."""
+    p = problem(78, LARGE, 1024, 64)
+    rows = p["a"].shape[0]
+    rng = np.random.default_rng(1)
+    p["off"] = rng.integers(-(1 << 31), 1 << 31, len(LARGE) + 1).astype(np.int32)
+    p["counts"] = rng.integers(-(1 << 31), 1 << 31, len(LARGE)).astype(np.int32)
+    run_raw(p, False)
+    p["off"][:] = 0
+    p["counts"][:] = rows                                             # every expert claims every row
+    run_raw(p, True)
+
+
 @pytest.mark.parametrize("silu", [False, True])
 def test_extreme_codes(silu):
     """-128 .. 127 at the largest sums, gates far out on both sides."""

@@ -180,3 +180,31 @@ def test_no_rows():
     assert q.shape == (0, 256) and s.shape == (0, 1) and ops.dequantize_rows(q, s).shape == (0, 256)
     got = ops.rms_norm_quantize(x, torch.ones(256, dtype=torch.bfloat16, device=xu.DEV), residual=x)
     assert [t.shape[0] for t in got] == [0, 0, 0]
+
+
+def test_more_rows_than_one_launch_takes():
+    """70 million rows: more threads than a launch has."""
+    rows = 70_000_000
+    free, _ = torch.cuda.mem_get_info()
+    if free < 8 << 30:
+        pytest.skip("needs 8 GiB of device memory")
+    x = torch.zeros((rows, 8), dtype=torch.bfloat16, device=xu.DEV)
+    at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, rows - 1], device=xu.DEV)
+    x[at] = rows_of(np.random.default_rng(2), 7, 8).to(xu.DEV)
+    q, s = ops.quantize_rows(x)
+    want_q, want_s = ops.quantize_rows(x[at])
+    assert torch.equal(q[at], want_q) and torch.equal(s[at], want_s)
+    q[at], s[at] = 0, 1.0
+    assert not bool(q.any()) and bool((s == 1.0).all())              # all other rows are rows of zeros
+
+
+def test_one_row_in_a_thousand_threads_is_the_same_as_among_many():
+    """Few rows take other launch shapes than many: the same codes either way."""
+    x = rows_of(np.random.default_rng(6), 300, 7168).to(xu.DEV)
+    g = torch.ones(7168, dtype=torch.bfloat16, device=xu.DEV)
+    for quant in ("int8", "e4m3"):
+        q, s = ops.quantize_rows(x, quant=quant)
+        for n in (1, 2, 255, 256, 257):
+            few_q, few_s = ops.quantize_rows(x[:n], quant=quant)
+            assert torch.equal(few_q.view(torch.uint8), q[:n].view(torch.uint8)) and torch.equal(few_s, s[:n])
+    assert len(ops.rms_norm_quantize(x[:1], g)) == 2
