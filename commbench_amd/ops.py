@@ -533,30 +533,35 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 def _quant_format(quant: str, width: int):
-    _require(quant in _QUANT_FORMATS, 'quant must be "int8" or "e4m3"')
-    _require(width > 0 and width % 8 == 0 and width <= QUANT_MAX_HIDDEN,
-             f"hidden must be a multiple of 8, at most {QUANT_MAX_HIDDEN}")
-    if quant == "e4m3":
-        _require(width % QUANT_BLOCK == 0, f"hidden must be a multiple of {QUANT_BLOCK} for e4m3")
-        return (*_QUANT_FORMATS[quant], width // QUANT_BLOCK)
-    return (*_QUANT_FORMATS[quant], 1)
+    """(format code, dtype of the codes, scales of a row)."""
+    found = _QUANT_FORMATS.get(quant)
+    _require(found is not None, 'quant must be "int8" or "e4m3"')
+    _require(width > 0 and width % 8 == 0 and width <= QUANT_MAX_HIDDEN, "hidden must be a multiple of 8, at most 32768")
+    if found[0] == 0:
+        return 0, found[1], 1
+    _require(width % QUANT_BLOCK == 0, "hidden must be a multiple of 128 for e4m3")
+    return 1, found[1], width // QUANT_BLOCK
 
 
-def _check_rows(x: torch.Tensor, name: str, device: Optional[torch.device] = None) -> None:
-    _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1)
-             and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0)) and x.data_ptr() % 16 == 0,
-             f"{name} must be a bf16 [rows, hidden] GPU tensor of 16-byte aligned rows")
-    _require(device is None or x.device == device, f"{name} must live on the device of x")
+def _check_rows(x: torch.Tensor, name: str):
+    """(rows, hidden, elements between rows, address) of a bf16 matrix of 16-byte aligned rows."""
+    if x.dtype is torch.bfloat16 and x.is_cuda and x.dim() == 2:
+        rows, hidden = x.shape
+        row_stride, stride = x.stride()
+        at = x.data_ptr()
+        if rows <= 1:
+            row_stride = hidden
+        if (stride == 1 or hidden == 1) and row_stride >= hidden and (rows <= 1 or row_stride % 8 == 0) and at % 16 == 0:
+            return rows, hidden, row_stride, at
+    raise ValueError(f"{name} must be a bf16 [rows, hidden] GPU tensor of 16-byte aligned rows")
 
 
-def _row_stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
-
-
-def _check_row_limit(row_limit: Optional[torch.Tensor], device: torch.device) -> None:
-    _require(row_limit is None or (row_limit.dtype == torch.int32 and row_limit.numel() == 1
-                                   and row_limit.device == device),
+def _check_row_limit(row_limit: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
+    if row_limit is None:
+        return None
+    _require(row_limit.dtype == torch.int32 and row_limit.numel() == 1 and row_limit.device == device,
              "row_limit must be one int32 on the rows' device")
+    return row_limit.data_ptr()
 
 
 def _empty_scales(rows: int, groups: int, device: torch.device, column_major: bool) -> torch.Tensor:
@@ -575,33 +580,33 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     columns, max|y| / 448); scales come as float32 [rows, groups], what dispatch takes.  Returns (q, scales),
     then the new residual stream bf16(h) when `residual` is given (written over it with
     `update_residual`), then bf16(y) with `normed`.  x and residual may be views with padded rows."""
-    _check_rows(x, "x")
-    T, H = x.shape
+    T, H, x_stride, x_at = _check_rows(x, "x")
     fmt, dtype, groups = _quant_format(quant, H)
     dev = x.device
-    _require(weight.dtype == torch.bfloat16 and weight.dim() == 1 and weight.shape[0] == H and weight.is_contiguous()
-             and weight.device == dev and weight.data_ptr() % 16 == 0, "weight must be contiguous bf16 [hidden] on the device of x")
+    g_at = weight.data_ptr()
+    _require(weight.dtype is torch.bfloat16 and weight.shape == (H,) and weight.is_contiguous() and weight.device == dev
+             and g_at % 16 == 0, "weight must be contiguous bf16 [hidden] on the device of x")
     _require(0.0 <= eps < float("inf"), "eps must be finite and not negative")
-    out_residual = None
+    out_residual = r_at = out_at = None
+    r_stride = 0
     if residual is not None:
-        _check_rows(residual, "residual", dev)
-        _require(residual.shape == x.shape, "residual must have the shape of x")
-        _require(not update_residual or residual.is_contiguous(), "a residual updated in place must be contiguous")
+        r_rows, r_hidden, r_stride, r_at = _check_rows(residual, "residual")
+        _require(r_rows == T and r_hidden == H and residual.device == dev, "residual must have the shape and device of x")
+        _require(not update_residual or r_stride == H, "a residual updated in place must be contiguous")
         out_residual = residual if update_residual else torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+        out_at = out_residual.data_ptr()
     else:
         _require(not update_residual, "update_residual needs a residual")
     q = torch.empty((T, H), dtype=dtype, device=dev)
     scales = _empty_scales(T, groups, dev, column_major_scales)
     out_normed = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if normed else None
-    _launch(dev, "mi_ep_rms_norm_quantize", x.data_ptr(), _row_stride(x), _ptr(residual),
-            _row_stride(residual) if residual is not None else 0, weight.data_ptr(),
-            struct.unpack("<I", struct.pack("<f", eps))[0], T, H, fmt, q.data_ptr(), scales.data_ptr(), *_scale_strides(scales),
-            _ptr(out_residual), _ptr(out_normed))
-    return tuple(t for t in (q, scales, out_residual, out_normed) if t is not None)
-
-
-def _scale_strides(scales: torch.Tensor) -> Tuple[int, int]:
-    return scales.stride(0), scales.stride(1)
+    row_stride, hidden_stride = scales.stride()
+    _launch(dev, "mi_ep_rms_norm_quantize", x_at, x_stride, r_at, r_stride, g_at,
+            struct.unpack("<I", struct.pack("<f", eps))[0], T, H, fmt, q.data_ptr(), scales.data_ptr(), row_stride, hidden_stride,
+            out_at, _ptr(out_normed))
+    if out_residual is None:
+        return (q, scales) if out_normed is None else (q, scales, out_normed)
+    return (q, scales, out_residual) if out_normed is None else (q, scales, out_residual, out_normed)
 
 
 def quantize_rows(x: torch.Tensor, quant: str = "int8", row_limit: Optional[torch.Tensor] = None,
@@ -609,14 +614,15 @@ def quantize_rows(x: torch.Tensor, quant: str = "int8", row_limit: Optional[torc
     """Rows of bf16 to 8 bits with scales, as rms_norm_quantize makes them: (q, scales).  With `row_limit`
     (one int32 on the device, e.g. handle.expert_offsets[-1:]) rows at and beyond it are left as they
     were: what a receive buffer holds behind its last row is not touched."""
-    _check_rows(x, "x")
-    rows, H = x.shape
+    rows, H, x_stride, x_at = _check_rows(x, "x")
     fmt, dtype, groups = _quant_format(quant, H)
-    _check_row_limit(row_limit, x.device)
-    q = torch.empty((rows, H), dtype=dtype, device=x.device)
-    scales = _empty_scales(rows, groups, x.device, column_major_scales)
-    _launch(x.device, "mi_ep_quantize_rows", x.data_ptr(), _row_stride(x), _ptr(row_limit), rows, H, fmt, q.data_ptr(),
-            scales.data_ptr(), *_scale_strides(scales))
+    dev = x.device
+    limit = _check_row_limit(row_limit, dev)
+    q = torch.empty((rows, H), dtype=dtype, device=dev)
+    scales = _empty_scales(rows, groups, dev, column_major_scales)
+    row_stride, hidden_stride = scales.stride()
+    _launch(dev, "mi_ep_quantize_rows", x_at, x_stride, limit, rows, H, fmt, q.data_ptr(), scales.data_ptr(), row_stride,
+            hidden_stride)
     return q, scales
 
 
@@ -624,16 +630,19 @@ def dequantize_rows(q: torch.Tensor, scales: torch.Tensor, row_limit: Optional[t
     """bf16(q * scale) of int8 rows with a scale each or float8_e4m3fn rows with a scale for each 128
     columns: an 8-bit payload (x, or recv_x after dispatch) for experts that compute in bf16.  `scales` may
     be any 2-D float32 view."""
-    _require(q.is_cuda and q.dim() == 2 and q.is_contiguous() and q.dtype in (torch.int8, torch.float8_e4m3fn),
+    dtype = q.dtype
+    _require((dtype is torch.int8 or dtype is torch.float8_e4m3fn) and q.is_cuda and q.dim() == 2 and q.is_contiguous(),
              "q must be a contiguous int8 or float8_e4m3fn [rows, hidden] GPU tensor")
     rows, H = q.shape
-    fmt, _, groups = _quant_format("int8" if q.dtype == torch.int8 else "e4m3", H)
-    _require(scales.dtype == torch.float32 and tuple(scales.shape) == (rows, groups) and scales.device == q.device
-             and min(scales.stride()) >= 0, "scales must be a float32 [rows, groups] tensor or view on the device of q")
-    _check_row_limit(row_limit, q.device)
-    out = torch.empty((rows, H), dtype=torch.bfloat16, device=q.device)
-    _launch(q.device, "mi_ep_dequantize_rows", q.data_ptr(), scales.data_ptr(), *_scale_strides(scales), _ptr(row_limit),
-            rows, H, fmt, out.data_ptr())
+    fmt, _, groups = _quant_format("int8" if dtype is torch.int8 else "e4m3", H)
+    dev = q.device
+    _require(scales.dtype is torch.float32 and scales.shape == (rows, groups) and scales.device == dev,
+             "scales must be a float32 [rows, groups] tensor or view on the device of q")
+    limit = _check_row_limit(row_limit, dev)
+    out = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
+    row_stride, hidden_stride = scales.stride()
+    _launch(dev, "mi_ep_dequantize_rows", q.data_ptr(), scales.data_ptr(), row_stride, hidden_stride, limit, rows, H, fmt,
+            out.data_ptr())
     return out
 
 
