@@ -60,6 +60,50 @@ def test_layer_against_64_bits(T, E, K, H, I, mask, kind, quantised):
     xu.check_within(xu.f64(call(on_gpu(p))), want, bound)
 
 
+FOLDS = [  # few routes for each expert, several for one of them; many for one, few for the others
+    (12, 64, 2, 160, 64, 0.0, "zipf"), (12, 64, 4, 272, 48, 0.1, "zipf"), (8, 512, 8, 48, 32, 0.0, "zipf"),
+    (40, 64, 4, 160, 64, 0.0, "zipf"), (40, 64, 4, 528, 144, 0.2, "zipf"), (128, 1024, 8, 32, 16, 0.0, "uniform")]
+
+
+@pytest.mark.parametrize("T,E,K,H,I,mask,kind", FOLDS)
+@pytest.mark.parametrize("quantised", [True, False])
+def test_experts_of_uneven_counts(T, E, K, H, I, mask, kind, quantised):
+    print(f"tokens {T} experts {E} slots {K} hidden {H} intermediate {I} masked {mask} {kind} int8 {quantised}", flush=True)
+    p = problem(T * 10 + H, T, E, K, H, I, quantised, mask, kind)
+    want, bound = reference(p)
+    xu.check_within(xu.f64(call(on_gpu(p))), want, bound)
+
+
+@pytest.mark.parametrize("T,E,expert", [(16, 512, 511), (17, 1024, 1023), (33, 1024, 0), (128, 64, 63)])
+@pytest.mark.parametrize("quantised", [True, False])
+def test_every_token_to_one_expert(T, E, expert, quantised):
+    """More routes than a pass over an expert's weights holds, where the mean of routes to an expert is tiny."""
+    p = problem(T + E, T, E, 2, 96, 48, quantised)
+    p["ids"][:, 0], p["ids"][:, 1] = expert, -1
+    p["ids"][T // 2, 1] = E - 1 - expert
+    want, bound = reference(p)
+    xu.check_within(xu.f64(call(on_gpu(p))), want, bound)
+
+
+@pytest.mark.parametrize("quantised", [True, False])
+def test_weights_behind_4_gib(quantised):
+    """The last expert's weights lie further than 32 bits of bytes from the first's."""
+    E, H, I, size = 700 if quantised else 350, 2560, 1280, 1 if quantised else 2
+    assert (E - 1) * 2 * I * H * size > 1 << 32
+    p = problem(29, 3, 2, 1, H, I, quantised)
+    p["ids"][:] = [[1], [0], [1]]
+    want, bound = reference(p)
+    g = on_gpu(p)
+    for name in ("w13", "w2", "s13", "s2"):
+        if g[name] is None:
+            continue
+        small, wide = g[name], torch.zeros((E, *g[name].shape[1:]), dtype=g[name].dtype, device=xu.DEV)
+        wide[0], wide[E - 1] = small[0], small[1]
+        g[name] = wide
+    g["ids"] = torch.where(g["ids"] == 1, E - 1, 0)
+    xu.check_within(xu.f64(call(g)), want, bound)
+
+
 @pytest.mark.parametrize("quantised", [True, False])
 def test_masked_ids_duplicates_and_tokens_without_a_route(quantised):
     T, E, K, H, I = 9, 5, 4, 160, 48
