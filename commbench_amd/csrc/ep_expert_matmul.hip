@@ -210,11 +210,16 @@ constexpr int kBigN = 256;       // channels of a tile: with kSilu 128 gate chan
 constexpr int kBlockRows = 64;   // a tile's rows come in pairs of 32-row blocks, one for each half of the waves
 constexpr int kMaxBlocks = 4;    // 256 rows: the accumulators fill the matrix units' own registers
 constexpr int kBigThreads = 256;
-constexpr int kStages = 4;
 constexpr int kRowGroup = 8;
-constexpr int kABytes = kMaxBlocks * kBlockRows * kBigK;     // 16 KiB: a stage is 64 bytes of k of the rows
-constexpr int kStageBytes = kABytes + kBigN * kBigK;         // and 16 KiB of the channels
-constexpr int kRingBytes = kStages * kStageBytes;            // 128 KiB
+// A stage of the ring is 64 bytes of k: of the channels (16 KiB), then of the rows (4 KiB a block).  Tiles of few rows
+// wait for memory and have room for more stages.
+constexpr int kBBytes = kBigN * kBigK;
+constexpr int kRingBytes = 128 * 1024;
+__host__ __device__ constexpr int stage_bytes_of(int blocks) { return kBBytes + blocks * kBlockRows * kBigK; }
+__host__ __device__ constexpr int stages_of(int blocks) { return blocks == 1 ? 6 : blocks == 2 ? 5 : 4; }
+static_assert(stages_of(1) * stage_bytes_of(1) <= kRingBytes && stages_of(2) * stage_bytes_of(2) <= kRingBytes &&
+                  stages_of(3) * stage_bytes_of(3) <= kRingBytes && stages_of(4) * stage_bytes_of(4) <= kRingBytes,
+              "the ring");
 constexpr int kEpiloguePitch = 64 * 2 + 16;                  // 64 columns of bf16, rows shifted by four banks
 constexpr int kEpilogueBytes = 32 * kEpiloguePitch;          // one wave's 32 rows
 constexpr int kTableAt = kRingBytes + 4 * kEpilogueBytes;    // row tiles before every thread's experts
@@ -261,19 +266,18 @@ struct BigMatmul {
         columns(kSilu ? args.out_features / 2 : args.out_features),
         steps((args.in_features + kBigK - 1) / kBigK) {}
 
-  // Load j of a stage: 16 rows of the channels, or 16 rows of the tokens.
-  __device__ __forceinline__ void load_b(const Place& at, int step, int j, bool inside) const {
-    const int to = lds_base + (step & (kStages - 1)) * kStageBytes + kABytes + (wave * 4 + j) * kChunkBytes;
+  // Load j of stage `step`, whose place in the ring is `slot`: 16 rows of the channels, or 16 rows of the tokens.
+  __device__ __forceinline__ void load_b(const Place& at, int slot, int step, int j, bool inside) const {
     const int row = (kSilu ? wave & 1 : wave) * 64 + at.row + j * 16;
-    load_to_lds(desc_b, to, inside ? row * K + at.piece : kOutside, step * kBigK);
+    load_to_lds(desc_b, lds_base + slot + (wave * 4 + j) * kChunkBytes, inside ? row * K + at.piece : kOutside, step * kBigK);
   }
-  __device__ __forceinline__ void load_a(const Place& at, int step, int j, bool inside) const {
-    const int to = lds_base + (step & (kStages - 1)) * kStageBytes + (j * 4 + wave) * kChunkBytes;
+  __device__ __forceinline__ void load_a(const Place& at, int slot, int step, int j, bool inside) const {
     const int row = (j * 4 + wave) * 16 + at.row;
-    load_to_lds(desc_a, to, inside ? row * K + at.piece : kOutside, step * kBigK);
+    load_to_lds(desc_a, lds_base + slot + kBBytes + (j * 4 + wave) * kChunkBytes, inside ? row * K + at.piece : kOutside,
+                step * kBigK);
   }
 
-  // Points the descriptors at a tile and starts its scales' and first three stages' loads.
+  // Points the descriptors at a tile and starts the loads of its scales and of its first stages, all but one of the ring's.
   __device__ __forceinline__ void start(const BigTile& tile, int scales_at) {
     const int b_rows = columns - tile.column < kColumns ? columns - tile.column : kColumns;
     const size_t channel = static_cast<size_t>(tile.expert) * a.out_features + (kSilu && wave >= 2 ? columns : 0) + tile.column;
@@ -288,13 +292,15 @@ struct BigMatmul {
     load_word_to_lds(descriptor_of(a.b_scales + channel, b_rows * 4), scales_at + kRowScaleBytes + wave * 256,
                      (kSilu ? row & 127 : row) * 4);
     const int blocks = (tile.rows + kBlockRows - 1) / kBlockRows;
-    for (int s = 0; s < 3 && s < steps; ++s) {
+    const int stages = stages_of(blocks) - 1;
+    for (int s = 0; s < stages && s < steps; ++s) {
       const bool inside = s * kBigK + at.piece < K;
+      const int slot = s * stage_bytes_of(blocks);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) load_b(at, s, j, inside);
+      for (int j = 0; j < 4; ++j) load_b(at, slot, s, j, inside);
 #pragma unroll
       for (int j = 0; j < kMaxBlocks; ++j)
-        if (j < blocks) load_a(at, s, j, inside);
+        if (j < blocks) load_a(at, slot, s, j, inside);
     }
   }
 
@@ -305,31 +311,33 @@ struct BigMatmul {
   // Fragment q of a half-step: four of channels, then the rows'.  Lane l takes row l % 32 of a block and piece
   // 2 * half + l / 32.
   template <int kBlocks>
-  __device__ __forceinline__ void read(const Place& at, Fragments<kBlocks>& f, int step, int half, int q) const {
-    const unsigned char* base = lds + (step & (kStages - 1)) * kStageBytes + (at.read_at ^ (half * 32));
+  __device__ __forceinline__ void read(const Place& at, Fragments<kBlocks>& f, int slot, int half, int q) const {
+    const unsigned char* base = lds + slot + (at.read_at ^ (half * 32));
     if (q < 4) {
       const int block = kSilu ? (q & 1) + nw * 2 + (q >> 1) * 4 : nw * 4 + q;
-      f.b[half][q] = *reinterpret_cast<const int4v*>(base + kABytes + block * 2048);
+      f.b[half][q] = *reinterpret_cast<const int4v*>(base + block * 2048);
     } else {
-      f.a[half][q - 4] = *reinterpret_cast<const int4v*>(base + (2 * (q - 4) + mw) * 2048);
+      f.a[half][q - 4] = *reinterpret_cast<const int4v*>(base + kBBytes + (2 * (q - 4) + mw) * 2048);
     }
   }
 
-  // Half a step: the products of one half's fragments; between them the reads of the next half's fragments
-  // and the loads of stage step + 3, of the channels in the first half and of the rows in the second.
+  // Half a step: the products of one half's fragments; between them, one to a product, the reads of the next
+  // half's fragments (in `from`) and the loads of the stage `ahead` (to `to`), of the channels in the first half and
+  // of the rows in the second.
   template <int kBlocks, int kHalf, bool kLoad>
-  __device__ __forceinline__ void half_step(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int step) const {
+  __device__ __forceinline__ void half_step(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int from, int to,
+                                            int ahead) const {
     constexpr int kLoads = !kLoad ? 0 : kHalf == 0 ? 4 : kBlocks;
     constexpr int kProducts = 4 * kBlocks, kReads = 4 + kBlocks, kItems = kReads + kLoads;
-    const bool inside = (step + 3) * kBigK + at.piece < K;
+    const bool inside = ahead * kBigK + at.piece < K;
 #pragma unroll
     for (int p = 0; p < kProducts; ++p) {
 #pragma unroll
       for (int i = p * kItems / kProducts; i < (p + 1) * kItems / kProducts; ++i) {
         const int loads_before = kLoads == 0 ? 0 : (i + 1) * kLoads / kItems;
         const bool is_load = kLoads != 0 && loads_before != i * kLoads / kItems;
-        if (is_load) kHalf == 0 ? load_b(at, step + 3, loads_before - 1, inside) : load_a(at, step + 3, loads_before - 1, inside);
-        else read<kBlocks>(at, f, kHalf == 0 ? step : step + 1, 1 - kHalf, i - loads_before);
+        if (is_load) kHalf == 0 ? load_b(at, to, ahead, loads_before - 1, inside) : load_a(at, to, ahead, loads_before - 1, inside);
+        else read<kBlocks>(at, f, from, 1 - kHalf, i - loads_before);
       }
       acc[p / 4][p % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[kHalf][p % 4], f.a[kHalf][p / 4], acc[p / 4][p % 4], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
@@ -348,31 +356,38 @@ struct BigMatmul {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[m][j] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
-    constexpr int kStageLoads = 4 + kBlocks;
-    if (steps > 2)
-      wait_and_meet<2 * kStageLoads + kStores>();
+    constexpr int kStages = stages_of(kBlocks), kStageBytes = stage_bytes_of(kBlocks), kStageLoads = 4 + kBlocks;
+    if (steps >= kStages - 1)
+      wait_and_meet<(kStages - 2) * kStageLoads + kStores>();
     else
       wait_and_meet<kStores>();
 #pragma unroll
     for (int q = 0; q < 4 + kBlocks; ++q) read<kBlocks>(at, f, 0, 0, q);
-    // The barrier in the middle of step s makes stage s + 1 visible, whose loads were issued in step s - 2 (those
-    // of step s - 1, four of step s and at first the previous tile's stores may still be on their way), and
-    // tells that every wave is done with reading stage s, whose place the loads of step s + 1 fill.
-    int step = 0;
-    for (; step < 2 && step + 3 < steps; ++step) {
-      half_step<kBlocks, 0, true>(at, f, acc, step);
-      wait_and_meet<kStageLoads + 4 + kStores>();
-      half_step<kBlocks, 1, true>(at, f, acc, step);
+    // The barrier in the middle of step s makes stage s + 1 visible (younger ones, four loads of step s and at first
+    // the previous tile's stores may still be on their way), and tells that every wave is done with reading stage
+    // s, whose place the loads of step s + 1 fill.
+    int step = 0, here = 0;
+    const auto after = [](int slot) { return slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes; };
+    const auto before = [](int slot) { return slot == 0 ? (kStages - 1) * kStageBytes : slot - kStageBytes; };
+    for (; step < kStages - 2 && step + kStages - 1 < steps; ++step, here = after(here)) {
+      half_step<kBlocks, 0, true>(at, f, acc, here, before(here), step + kStages - 1);
+      wait_and_meet<(kStages - 3) * kStageLoads + 4 + kStores>();
+      half_step<kBlocks, 1, true>(at, f, acc, after(here), before(here), step + kStages - 1);
     }
-    for (; step + 3 < steps; ++step) {
-      half_step<kBlocks, 0, true>(at, f, acc, step);
-      wait_and_meet<kStageLoads + 4>();
-      half_step<kBlocks, 1, true>(at, f, acc, step);
+    for (; step + kStages - 1 < steps; ++step, here = after(here)) {
+      half_step<kBlocks, 0, true>(at, f, acc, here, before(here), step + kStages - 1);
+      wait_and_meet<(kStages - 3) * kStageLoads + 4>();
+      half_step<kBlocks, 1, true>(at, f, acc, after(here), before(here), step + kStages - 1);
     }
-    for (; step < steps; ++step) {
-      half_step<kBlocks, 0, false>(at, f, acc, step);
-      wait_and_meet<0>();
-      half_step<kBlocks, 1, false>(at, f, acc, step);
+    for (; step < steps; ++step, here = after(here)) {
+      half_step<kBlocks, 0, false>(at, f, acc, here, 0, 0);
+      switch (steps - step) {  // stages behind the next one: steps - step - 2, none of them younger than a load of this loop
+        case 5: wait_and_meet<3 * kStageLoads>(); break;
+        case 4: wait_and_meet<2 * kStageLoads>(); break;
+        case 3: wait_and_meet<kStageLoads>(); break;
+        default: wait_and_meet<0>(); break;
+      }
+      half_step<kBlocks, 1, false>(at, f, acc, after(here), 0, 0);
     }
     // The next tile's loads run during this one's epilogue.
     if (has_next) start(next, next_scales_at);
