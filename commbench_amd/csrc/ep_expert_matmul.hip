@@ -62,20 +62,18 @@ __device__ __forceinline__ int lds_address(const unsigned char* p) {
 // v / (1 + exp(-v)); the reciprocal instruction is off by one unit in the last place at most.
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 
-// A lane's part in the loads and reads of a stage.  A stage holds rows of 64 bytes, two to a 128-byte line; the
-// line's eight 16-byte pieces are permuted by exclusive or with the line number, so that 8 lanes reading one
-// piece of 8 rows meet all banks.  A load instruction fills 16 rows in order; lane l of it fetches the piece
-// that belongs at l.
+// A lane's part in the loads and reads of a stage.  A stage holds rows of 64 bytes; the four 16-byte pieces of a row are
+// permuted by exclusive or with a quarter of its number, so that 16 lanes reading one piece of 16 rows meet all 64
+// banks.  A load instruction fills 16 rows in order; lane l of it fetches the piece that belongs at l.
 struct Place {
   int piece, row, read_at;
   __device__ __forceinline__ explicit Place(int lane) {
-    const int logical = (lane & 7) ^ (lane >> 3), r = lane & 31;
-    piece = (logical & 3) * 16;
-    row = (lane >> 3) * 2 + (logical >> 2);
-    read_at = (r >> 1) * 128 + ((((r & 1) * 4 + (lane >> 5)) ^ ((r >> 1) & 7)) * 16);
+    const int r = lane & 31;
+    piece = ((lane & 3) ^ (lane >> 4)) * 16;
+    row = lane >> 2;
+    read_at = r * 64 + (((lane >> 5) ^ ((r >> 2) & 3)) * 16);
   }
 };
-
 
 // ---- small tiles: 64 rows by 64 columns, for problems of few tiles --------------------------------------
 constexpr int kTileM = 64, kTileN = 64;
