@@ -4,6 +4,8 @@
 //   out = bf16(c)   or, gate and up in one product,   out[m, i] = bf16(silu(c[m, i]) * c[m, I + i])
 // The sum over k is exact in 32-bit integers (|a|, |b| <= 128 and k < 2^17).
 #include <atomic>
+#include <type_traits>
+
 #include "ep_device.h"
 
 namespace mi_ep {
@@ -11,7 +13,7 @@ namespace {
 
 typedef int int4v __attribute__((ext_vector_type(4)));
 
-constexpr int kBigK = 64;                                      // bytes of k in a stage
+constexpr int kStageK = 128;                                   // bytes of k in a stage
 constexpr int kChunkBytes = 1024;                              // what one load instruction of a wave moves
 constexpr int kOutside = static_cast<int>(0x80000000u);        // an offset beyond every descriptor
 
@@ -62,17 +64,19 @@ __device__ __forceinline__ int lds_address(const unsigned char* p) {
 // v / (1 + exp(-v)); the reciprocal instruction is off by one unit in the last place at most.
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 
-// A lane's part in the loads and reads of a stage.  A stage holds rows of 64 bytes; the four 16-byte pieces of a row are
-// permuted by exclusive or with a quarter of its number, so that 16 lanes reading one piece of 16 rows meet all 64
-// banks.  A load instruction fills 16 rows in order; lane l of it fetches the piece that belongs at l.
+// A lane's part in the loads and reads of a stage.  A stage holds rows of 128 bytes, whole cache lines (of half lines
+// the memory delivers a fifth less); the eight 16-byte pieces of a row are permuted by exclusive or with half its
+// number, so that 16 lanes reading one piece of 16 rows meet all 64 banks.  A load instruction fills eight rows in
+// order; lane l of it fetches the piece that belongs at l, which in every other eight rows is the one 64 bytes away.
 struct Place {
   int piece, row, read_at;
   __device__ __forceinline__ explicit Place(int lane) {
     const int r = lane & 31;
-    piece = ((lane & 3) ^ (lane >> 4)) * 16;
-    row = lane >> 2;
-    read_at = r * 64 + (((lane >> 5) ^ ((r >> 2) & 3)) * 16);
+    piece = ((lane & 7) ^ (lane >> 4)) * 16;
+    row = lane >> 3;
+    read_at = r * 128 + (((lane >> 5) ^ ((r >> 1) & 7)) * 16);
   }
+  __device__ __forceinline__ int piece_of(int eight) const { return piece ^ ((eight & 1) * 64); }
 };
 
 // ---- small tiles: 64 rows by 64 columns, for problems of few tiles --------------------------------------
@@ -126,9 +130,9 @@ __device__ __forceinline__ RowTile find_row_tile(const ExpertMatmulArgs& a, int 
 template <bool kSilu>
 __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(const ExpertMatmulArgs a) {
   constexpr int kSets = kSilu ? 2 : 1;
-  constexpr int kRing = 6;
-  constexpr int kABytes = kTileM * kBigK, kStage = kABytes + kSets * kTileN * kBigK;
-  constexpr int kLoads = 1 + kSets;  // of a wave for a stage
+  constexpr int kRing = 3;
+  constexpr int kABytes = kTileM * kStageK, kStage = kABytes + kSets * kTileN * kStageK;
+  constexpr int kLoads = 2 * (1 + kSets);  // of a wave for a stage
   __shared__ __align__(1024) unsigned char ring[kRing * kStage];
   const RowTile tile = find_row_tile(a, static_cast<int>(blockIdx.y));
   if (tile.rows <= 0) return;
@@ -138,23 +142,27 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
   const int lane = lane_id(), r = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int mw = wave & 1, nw = wave >> 1;
-  const int steps = (K + kBigK - 1) / kBigK;
+  const int steps = (K + kStageK - 1) / kStageK;
   const Place at(lane);
   const int b_rows = columns - n0 < kTileN ? columns - n0 : kTileN;
   const size_t channel = static_cast<size_t>(tile.expert) * a.out_features + n0;
   const int4v desc_a = descriptor_of(a.a + static_cast<size_t>(tile.first) * K, tile.rows * K);
   const int4v desc_b = descriptor_of(a.b + channel * K, b_rows * K);
   const int4v desc_up = kSilu ? descriptor_of(a.b + (channel + columns) * K, b_rows * K) : desc_b;
-  const int offset = (wave * 16 + at.row) * K + at.piece;
+  const int offset = (wave * 16 + at.row) * K;
   const int ring_base = lds_address(ring);
   int load_slot = 0;
   const auto load_stage = [&](int step) {  // steps behind the last load nothing, but count
-    const int k0 = step < steps ? step * kBigK : 0;
-    const int from = step * kBigK + at.piece < K ? offset : kOutside;
-    const int to = ring_base + load_slot * kStage + wave * kChunkBytes;
-    load_to_lds(desc_a, to, from, k0);
-    load_to_lds(desc_b, to + kABytes, from, k0);
-    if constexpr (kSilu) load_to_lds(desc_up, to + kABytes + kTileN * kBigK, from, k0);
+    const int k0 = step < steps ? step * kStageK : 0;
+    const int to = ring_base + load_slot * kStage + wave * 2 * kChunkBytes;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int piece = at.piece_of(j);
+      const int from = step * kStageK + piece < K ? offset + j * 8 * K + piece : kOutside;
+      load_to_lds(desc_a, to + j * kChunkBytes, from, k0);
+      load_to_lds(desc_b, to + kABytes + j * kChunkBytes, from, k0);
+      if constexpr (kSilu) load_to_lds(desc_up, to + kABytes + kTileN * kStageK + j * kChunkBytes, from, k0);
+    }
     load_slot = load_slot + 1 == kRing ? 0 : load_slot + 1;
   };
 #pragma unroll
@@ -170,12 +178,12 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
     load_stage(step + kRing - 1);
     const unsigned char* stage = ring + slot * kStage;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const unsigned char* base = stage + (at.read_at ^ (half * 32));
-      const int4v rows = *reinterpret_cast<const int4v*>(base + mw * 2048);
+    for (int quarter = 0; quarter < 4; ++quarter) {
+      const unsigned char* base = stage + (at.read_at ^ (quarter * 32));
+      const int4v rows = *reinterpret_cast<const int4v*>(base + mw * 32 * kStageK);
 #pragma unroll
       for (int s = 0; s < kSets; ++s) {
-        const int4v channels = *reinterpret_cast<const int4v*>(base + kABytes + s * kTileN * kBigK + nw * 2048);
+        const int4v channels = *reinterpret_cast<const int4v*>(base + kABytes + (s * kTileN + nw * 32) * kStageK);
         acc[s] = __builtin_amdgcn_mfma_i32_32x32x32_i8(channels, rows, acc[s], 0, 0, 0);
       }
     }
@@ -209,16 +217,16 @@ constexpr int kBlockRows = 64;   // a tile's rows come in pairs of 32-row blocks
 constexpr int kMaxBlocks = 4;    // 256 rows: the accumulators fill the matrix units' own registers
 constexpr int kBigThreads = 256;
 constexpr int kRowGroup = 8;
-// A stage of the ring is 64 bytes of k: of the channels (16 KiB), then of the rows (4 KiB a block).  Tiles of few rows
-// wait for memory and have room for more stages.
-constexpr int kBBytes = kBigN * kBigK;
-constexpr int kRingBytes = 128 * 1024;
-__host__ __device__ constexpr int stage_bytes_of(int blocks) { return kBBytes + blocks * kBlockRows * kBigK; }
-__host__ __device__ constexpr int stages_of(int blocks) { return blocks == 1 ? 6 : blocks == 2 ? 5 : 4; }
+// A stage of the ring is 128 bytes of k: of the channels (32 KiB), then of the rows (8 KiB for 64 of them).  Tiles of few
+// rows wait for memory and have room for a third stage.
+constexpr int kBBytes = kBigN * kStageK;
+constexpr int kRingBytes = 144 * 1024;
+__host__ __device__ constexpr int stage_bytes_of(int blocks) { return kBBytes + blocks * kBlockRows * kStageK; }
+__host__ __device__ constexpr int stages_of(int blocks) { return blocks <= 2 ? 3 : 2; }
 static_assert(stages_of(1) * stage_bytes_of(1) <= kRingBytes && stages_of(2) * stage_bytes_of(2) <= kRingBytes &&
                   stages_of(3) * stage_bytes_of(3) <= kRingBytes && stages_of(4) * stage_bytes_of(4) <= kRingBytes,
               "the ring");
-constexpr int kEpiloguePitch = 64 * 2 + 16;                  // 64 columns of bf16, rows shifted by four banks
+constexpr int kEpiloguePitch = 32 * 2 + 16;                  // 32 columns of bf16, rows shifted by four banks
 constexpr int kEpilogueBytes = 32 * kEpiloguePitch;          // one wave's 32 rows
 constexpr int kTableAt = kRingBytes + 4 * kEpilogueBytes;    // row tiles before every thread's experts
 constexpr int kRowScaleBytes = kMaxBlocks * kBlockRows * 4;
@@ -262,20 +270,21 @@ struct BigMatmul {
         nw(wave >> 1),
         K(args.in_features),
         columns(kSilu ? args.out_features / 2 : args.out_features),
-        steps((args.in_features + kBigK - 1) / kBigK) {}
+        steps((args.in_features + kStageK - 1) / kStageK) {}
 
-  // Load j of stage `step`, whose place in the ring is `slot`: 16 rows of the channels, or 16 rows of the tokens.
-  __device__ __forceinline__ void load_b(const Place& at, int slot, int step, int j, bool inside) const {
-    const int row = (kSilu ? wave & 1 : wave) * 64 + at.row + j * 16;
-    load_to_lds(desc_b, lds_base + slot + (wave * 4 + j) * kChunkBytes, inside ? row * K + at.piece : kOutside, step * kBigK);
+  // Load j of stage `step`, whose place in the ring is `slot`: eight rows of the channels, or of the tokens.
+  __device__ __forceinline__ void load_b(const Place& at, int slot, int step, int j) const {
+    const int row = (kSilu ? wave & 1 : wave) * 64 + at.row + j * 8, piece = at.piece_of(j);
+    load_to_lds(desc_b, lds_base + slot + (wave * 8 + j) * kChunkBytes,
+                step * kStageK + piece < K ? row * K + piece : kOutside, step * kStageK);
   }
-  __device__ __forceinline__ void load_a(const Place& at, int slot, int step, int j, bool inside) const {
-    const int row = (j * 4 + wave) * 16 + at.row;
-    load_to_lds(desc_a, lds_base + slot + kBBytes + (j * 4 + wave) * kChunkBytes, inside ? row * K + at.piece : kOutside,
-                step * kBigK);
+  __device__ __forceinline__ void load_a(const Place& at, int slot, int step, int j) const {
+    const int eight = (j >> 1) * 8 + wave * 2 + (j & 1), piece = at.piece_of(j);
+    load_to_lds(desc_a, lds_base + slot + kBBytes + eight * kChunkBytes,
+                step * kStageK + piece < K ? (eight * 8 + at.row) * K + piece : kOutside, step * kStageK);
   }
 
-  // Points the descriptors at a tile and starts the loads of its scales and of its first stages, all but one of the ring's.
+  // Points the descriptors at a tile and starts the loads of its scales and of its first stages, as many as the ring holds.
   __device__ __forceinline__ void start(const BigTile& tile, int scales_at) {
     const int b_rows = columns - tile.column < kColumns ? columns - tile.column : kColumns;
     const size_t channel = static_cast<size_t>(tile.expert) * a.out_features + (kSilu && wave >= 2 ? columns : 0) + tile.column;
@@ -290,15 +299,14 @@ struct BigMatmul {
     load_word_to_lds(descriptor_of(a.b_scales + channel, b_rows * 4), scales_at + kRowScaleBytes + wave * 256,
                      (kSilu ? row & 127 : row) * 4);
     const int blocks = (tile.rows + kBlockRows - 1) / kBlockRows;
-    const int stages = stages_of(blocks) - 1;
+    const int stages = stages_of(blocks);
     for (int s = 0; s < stages && s < steps; ++s) {
-      const bool inside = s * kBigK + at.piece < K;
       const int slot = s * stage_bytes_of(blocks);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) load_b(at, slot, s, j, inside);
+      for (int j = 0; j < 8; ++j) load_b(at, slot, s, j);
 #pragma unroll
-      for (int j = 0; j < kMaxBlocks; ++j)
-        if (j < blocks) load_a(at, slot, s, j, inside);
+      for (int j = 0; j < 2 * kMaxBlocks; ++j)
+        if (j < 2 * blocks) load_a(at, slot, s, j);
     }
   }
 
@@ -306,38 +314,38 @@ struct BigMatmul {
   struct Fragments {
     int4v a[2][kBlocks], b[2][4];
   };
-  // Fragment q of a half-step: four of channels, then the rows'.  Lane l takes row l % 32 of a block and piece
-  // 2 * half + l / 32.
+  // Fragment i of a quarter of a stage: four of channels, then the rows'.  Lane l takes row l % 32 of a block and
+  // piece 2 * quarter + l / 32.
   template <int kBlocks>
-  __device__ __forceinline__ void read(const Place& at, Fragments<kBlocks>& f, int slot, int half, int q) const {
-    const unsigned char* base = lds + slot + (at.read_at ^ (half * 32));
-    if (q < 4) {
-      const int block = kSilu ? (q & 1) + nw * 2 + (q >> 1) * 4 : nw * 4 + q;
-      f.b[half][q] = *reinterpret_cast<const int4v*>(base + block * 2048);
+  __device__ __forceinline__ void read(const Place& at, Fragments<kBlocks>& f, int slot, int quarter, int i) const {
+    const unsigned char* base = lds + slot + (at.read_at ^ (quarter * 32));
+    if (i < 4) {
+      const int block = kSilu ? (i & 1) + nw * 2 + (i >> 1) * 4 : nw * 4 + i;
+      f.b[quarter & 1][i] = *reinterpret_cast<const int4v*>(base + block * 32 * kStageK);
     } else {
-      f.a[half][q - 4] = *reinterpret_cast<const int4v*>(base + kBBytes + (2 * (q - 4) + mw) * 2048);
+      f.a[quarter & 1][i - 4] = *reinterpret_cast<const int4v*>(base + kBBytes + (2 * (i - 4) + mw) * 32 * kStageK);
     }
   }
 
-  // Half a step: the products of one half's fragments; between them, one to a product, the reads of the next
-  // half's fragments (in `from`) and the loads of the stage `ahead` (to `to`), of the channels in the first half and
-  // of the rows in the second.
-  template <int kBlocks, int kHalf, bool kLoad>
-  __device__ __forceinline__ void half_step(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int from, int to,
-                                            int ahead) const {
-    constexpr int kLoads = !kLoad ? 0 : kHalf == 0 ? 4 : kBlocks;
-    constexpr int kProducts = 4 * kBlocks, kReads = 4 + kBlocks, kItems = kReads + kLoads;
-    const bool inside = ahead * kBigK + at.piece < K;
+  enum Loads { kNone, kChannels, kRows };
+  // A quarter of a stage's products; between them, spread over them, the reads of the next quarter's fragments (from
+  // the stage in `from`, or with kRead false none) and the loads of a part of stage `ahead` (to `to`).
+  template <int kBlocks, int kQuarter, Loads kLoad, bool kRead = true>
+  __device__ __forceinline__ void quarter(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int from, int to,
+                                          int ahead) const {
+    constexpr int kLoads = kLoad == kNone ? 0 : kLoad == kChannels ? 8 : 2 * kBlocks;
+    constexpr int kProducts = 4 * kBlocks, kItems = (kRead ? 4 + kBlocks : 0) + kLoads;
 #pragma unroll
     for (int p = 0; p < kProducts; ++p) {
 #pragma unroll
       for (int i = p * kItems / kProducts; i < (p + 1) * kItems / kProducts; ++i) {
         const int loads_before = kLoads == 0 ? 0 : (i + 1) * kLoads / kItems;
         const bool is_load = kLoads != 0 && loads_before != i * kLoads / kItems;
-        if (is_load) kHalf == 0 ? load_b(at, to, ahead, loads_before - 1, inside) : load_a(at, to, ahead, loads_before - 1, inside);
-        else read<kBlocks>(at, f, from, 1 - kHalf, i - loads_before);
+        if (is_load) kLoad == kChannels ? load_b(at, to, ahead, loads_before - 1) : load_a(at, to, ahead, loads_before - 1);
+        else read<kBlocks>(at, f, from, (kQuarter + 1) & 3, i - loads_before);
       }
-      acc[p / 4][p % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[kHalf][p % 4], f.a[kHalf][p / 4], acc[p / 4][p % 4], 0, 0, 0);
+      constexpr int h = kQuarter & 1;
+      acc[p / 4][p % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[h][p % 4], f.a[h][p / 4], acc[p / 4][p % 4], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -354,44 +362,51 @@ struct BigMatmul {
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[m][j] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
-    constexpr int kStages = stages_of(kBlocks), kStageBytes = stage_bytes_of(kBlocks), kStageLoads = 4 + kBlocks;
-    if (steps >= kStages - 1)
-      wait_and_meet<(kStages - 2) * kStageLoads + kStores>();
+    constexpr int kStages = stages_of(kBlocks), kStageBytes = stage_bytes_of(kBlocks), kStageLoads = 8 + 2 * kBlocks;
+    if (steps >= kStages)
+      wait_and_meet<(kStages - 1) * kStageLoads + kStores>();
     else
       wait_and_meet<kStores>();
 #pragma unroll
-    for (int q = 0; q < 4 + kBlocks; ++q) read<kBlocks>(at, f, 0, 0, q);
-    // The barrier in the middle of step s makes stage s + 1 visible (younger ones, four loads of step s and at first
-    // the previous tile's stores may still be on their way), and tells that every wave is done with reading stage
-    // s, whose place the loads of step s + 1 fill.
+    for (int i = 0; i < 4 + kBlocks; ++i) read<kBlocks>(at, f, 0, 0, i);
+    quarter<kBlocks, 0, kNone>(at, f, acc, 0, 0, 0);
+    quarter<kBlocks, 1, kNone>(at, f, acc, 0, 0, 0);
+    quarter<kBlocks, 2, kNone>(at, f, acc, 0, 0, 0);
+    // The barrier behind the third quarter of stage s makes stage s + 1 visible (younger ones and at first the previous
+    // tile's stores may still be on their way), and tells that every wave has read all of stage s, whose place stage
+    // s + kStages then fills.
     int step = 0, here = 0;
     const auto after = [](int slot) { return slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes; };
-    const auto before = [](int slot) { return slot == 0 ? (kStages - 1) * kStageBytes : slot - kStageBytes; };
-    for (; step < kStages - 2 && step + kStages - 1 < steps; ++step, here = after(here)) {
-      half_step<kBlocks, 0, true>(at, f, acc, here, before(here), step + kStages - 1);
-      wait_and_meet<(kStages - 3) * kStageLoads + 4 + kStores>();
-      half_step<kBlocks, 1, true>(at, f, acc, after(here), before(here), step + kStages - 1);
+    const auto go_on = [&](auto load) {
+      constexpr bool kLoad = decltype(load)::value;
+      const int next_slot = after(here), ahead = step + kStages;
+      quarter<kBlocks, 3, kLoad ? kChannels : kNone>(at, f, acc, next_slot, here, ahead);
+      quarter<kBlocks, 0, kLoad ? kRows : kNone>(at, f, acc, next_slot, here, ahead);
+      quarter<kBlocks, 1, kNone>(at, f, acc, next_slot, 0, 0);
+      quarter<kBlocks, 2, kNone>(at, f, acc, next_slot, 0, 0);
+      ++step;
+      here = next_slot;
+    };
+    while (step < kStages - 1 && step + kStages < steps) {
+      wait_and_meet<(kStages - 2) * kStageLoads + kStores>();
+      go_on(std::true_type{});
     }
-    for (; step + kStages - 1 < steps; ++step, here = after(here)) {
-      half_step<kBlocks, 0, true>(at, f, acc, here, before(here), step + kStages - 1);
-      wait_and_meet<(kStages - 3) * kStageLoads + 4>();
-      half_step<kBlocks, 1, true>(at, f, acc, after(here), before(here), step + kStages - 1);
+    while (step + kStages < steps) {
+      wait_and_meet<(kStages - 2) * kStageLoads>();
+      go_on(std::true_type{});
     }
-    for (; step < steps; ++step, here = after(here)) {
-      half_step<kBlocks, 0, false>(at, f, acc, here, 0, 0);
-      switch (steps - step) {  // stages behind the next one: steps - step - 2, none of them younger than a load of this loop
-        case 5: wait_and_meet<3 * kStageLoads>(); break;
-        case 4: wait_and_meet<2 * kStageLoads>(); break;
-        case 3: wait_and_meet<kStageLoads>(); break;
-        default: wait_and_meet<0>(); break;
-      }
-      half_step<kBlocks, 1, false>(at, f, acc, after(here), 0, 0);
+    while (step + 1 < steps) {  // steps - step - 2 stages are behind the next one
+      if (steps - step > 2) wait_and_meet<(kStages - 2) * kStageLoads>();
+      else wait_and_meet<0>();
+      go_on(std::false_type{});
     }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    quarter<kBlocks, 3, kNone, false>(at, f, acc, 0, 0, 0);
     // The next tile's loads run during this one's epilogue.
     if (has_next) start(next, next_scales_at);
 
     // Lane l holds row l % 32 of a block and channels 8 g + 4 (l / 32) + 0..3; through the wave's own piece of
-    // LDS they become rows of 64 columns, stored 16 bytes a lane.
+    // LDS they become rows of 32 columns, stored 16 bytes a lane.
     const int lane = fresh(this->lane), r = lane & 31;
     unsigned char* mine = lds + kRingBytes + wave * kEpilogueBytes;
     const float* row_scales = reinterpret_cast<const float*>(lds + (scales_at - lds_base));
@@ -402,32 +417,28 @@ struct BigMatmul {
       const int row0 = (2 * m + mw) * 32;
       const float row_scale = row_scales[row0 + r];
 #pragma unroll
-      for (int part = 0; part < (kSilu ? 1 : 2); ++part) {
-        const int column0 = nw * (kSilu ? 64 : 128) + part * 64;  // in the tile
+      for (int j = 0; j < (kSilu ? 2 : 4); ++j) {
+        const int column0 = nw * (kSilu ? 64 : 128) + j * 32;  // in the tile
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          const int j = part * 2 + jj;
+        for (int g = 0; g < 4; ++g) {
+          const int c = g * 8 + (lane >> 5) * 4;
+          const float4 s4 = *reinterpret_cast<const float4*>(b_scales + column0 + c);
+          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+          float o[4];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int c = jj * 32 + g * 8 + (lane >> 5) * 4;
-            const float4 s4 = *reinterpret_cast<const float4*>(b_scales + column0 + c);
-            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
-            float o[4];
+          for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(acc[m][j][g * 4 + i]) * (row_scale * s[i]);
+          if constexpr (kSilu) {
+            const float4 t4 = *reinterpret_cast<const float4*>(b_scales + 128 + column0 + c);
+            const float u[4] = {t4.x, t4.y, t4.z, t4.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(acc[m][j][g * 4 + i]) * (row_scale * s[i]);
-            if constexpr (kSilu) {
-              const float4 t4 = *reinterpret_cast<const float4*>(b_scales + 128 + column0 + c);
-              const float u[4] = {t4.x, t4.y, t4.z, t4.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + 2) & 3][g * 4 + i]) * (row_scale * u[i]));
-            }
-            *reinterpret_cast<uint2*>(mine + r * kEpiloguePitch + c * 2) = uint2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])};
+            for (int i = 0; i < 4; ++i)
+              o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + 2) & 3][g * 4 + i]) * (row_scale * u[i]));
           }
+          *reinterpret_cast<uint2*>(mine + r * kEpiloguePitch + c * 2) = uint2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])};
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int local = q * 8 + (lane >> 3), c = (lane & 7) * 8;
+        for (int q = 0; q < 2; ++q) {
+          const int local = q * 16 + (lane >> 2), c = (lane & 3) * 8;
           const vec16 v = *reinterpret_cast<const vec16*>(mine + local * kEpiloguePitch + c * 2);
           const int column = tile.column + column0 + c;
           __builtin_amdgcn_raw_buffer_store_b128(v, out, column < columns ? ((row0 + local) * columns + column) * 2 : kOutside, 0, 0);
