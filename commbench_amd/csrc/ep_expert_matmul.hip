@@ -226,9 +226,8 @@ __host__ __device__ constexpr int stages_of(int blocks) { return blocks <= 2 ? 3
 static_assert(stages_of(1) * stage_bytes_of(1) <= kRingBytes && stages_of(2) * stage_bytes_of(2) <= kRingBytes &&
                   stages_of(3) * stage_bytes_of(3) <= kRingBytes && stages_of(4) * stage_bytes_of(4) <= kRingBytes,
               "the ring");
-constexpr int kEpiloguePitch = 32 * 2 + 16;                  // 32 columns of bf16, rows shifted by four banks
-constexpr int kEpilogueBytes = 32 * kEpiloguePitch;          // one wave's 32 rows
-constexpr int kTableAt = kRingBytes + 4 * kEpilogueBytes;    // row tiles before every thread's experts
+constexpr int kOutputPolicy = kCachePolicyStreaming | kCachePolicyDeviceScope;
+constexpr int kTableAt = kRingBytes;    // row tiles before every thread's experts
 constexpr int kRowScaleBytes = kMaxBlocks * kBlockRows * 4;
 constexpr int kScaleBytes = kRowScaleBytes + kBigN * 4;
 constexpr int kScalesAt = kTableAt + (kBigThreads + 4) * 4;  // two tiles' row and channel scales
@@ -405,45 +404,59 @@ struct BigMatmul {
     // The next tile's loads run during this one's epilogue.
     if (has_next) start(next, next_scales_at);
 
-    // Lane l holds row l % 32 of a block and channels 8 g + 4 (l / 32) + 0..3; through the wave's own piece of
-    // LDS they become rows of 32 columns, stored 16 bytes a lane.
+    // Lane l holds row l % 32 of a block and channels 8 g + 4 (l / 32) + 0..3.
     const int lane = fresh(this->lane), r = lane & 31;
-    unsigned char* mine = lds + kRingBytes + wave * kEpilogueBytes;
     const float* row_scales = reinterpret_cast<const float*>(lds + (scales_at - lds_base));
     const float* b_scales = row_scales + kRowScaleBytes / 4;
     const __amdgpu_buffer_rsrc_t out = out_rows(tile);
+    const int store_row = lane & 15, store_column = ((lane >> 5) + ((lane >> 3) & 2)) * 8;
+    float row_scale[kBlocks];
 #pragma unroll
-    for (int m = 0; m < kBlocks; ++m) {
-      const int row0 = (2 * m + mw) * 32;
-      const float row_scale = row_scales[row0 + r];
+    for (int m = 0; m < kBlocks; ++m) row_scale[m] = row_scales[(2 * m + mw) * 32 + r];
 #pragma unroll
-      for (int j = 0; j < (kSilu ? 2 : 4); ++j) {
-        const int column0 = nw * (kSilu ? 64 : 128) + j * 32;  // in the tile
+    for (int j = 0; j < (kSilu ? 2 : 4); ++j) {
+      const int column0 = nw * (kSilu ? 64 : 128) + j * 32;  // in the tile
+      float4 s[4], u[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        s[g] = *reinterpret_cast<const float4*>(b_scales + column0 + g * 8 + (lane >> 5) * 4);
+        if constexpr (kSilu) u[g] = *reinterpret_cast<const float4*>(b_scales + 128 + column0 + g * 8 + (lane >> 5) * 4);
+      }
+      const int column = tile.column + column0 + store_column;
+#pragma unroll
+      for (int m = 0; m < kBlocks; ++m) {
+        uint32_t w[4][2];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int c = g * 8 + (lane >> 5) * 4;
-          const float4 s4 = *reinterpret_cast<const float4*>(b_scales + column0 + c);
-          const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+          const float sg[4] = {s[g].x, s[g].y, s[g].z, s[g].w};
           float o[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(acc[m][j][g * 4 + i]) * (row_scale * s[i]);
+          for (int i = 0; i < 4; ++i) o[i] = static_cast<float>(acc[m][j][g * 4 + i]) * (row_scale[m] * sg[i]);
           if constexpr (kSilu) {
-            const float4 t4 = *reinterpret_cast<const float4*>(b_scales + 128 + column0 + c);
-            const float u[4] = {t4.x, t4.y, t4.z, t4.w};
+            const float ug[4] = {u[g].x, u[g].y, u[g].z, u[g].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + 2) & 3][g * 4 + i]) * (row_scale * u[i]));
+              o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + 2) & 3][g * 4 + i]) * (row_scale[m] * ug[i]));
           }
-          *reinterpret_cast<uint2*>(mine + r * kEpiloguePitch + c * 2) = uint2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])};
+          w[g][0] = to_bf16_pair(o[0], o[1]);
+          w[g][1] = to_bf16_pair(o[2], o[3]);
         }
+        // Exchanges between the halves of the wave give a lane eight columns in a row: l < 32 those of g = 0 (2), the others those
+        // of g = 1 (3); between groups of 16 lanes, 16 rows of 64 bytes to a store.
+        vec16 first, second;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int local = q * 16 + (lane >> 2), c = (lane & 3) * 8;
-          const vec16 v = *reinterpret_cast<const vec16*>(mine + local * kEpiloguePitch + c * 2);
-          const int column = tile.column + column0 + c;
-          __builtin_amdgcn_raw_buffer_store_b128(v, out, column < columns ? ((row0 + local) * columns + column) * 2 : kOutside, 0, 0);
+        for (int i = 0; i < 2; ++i) {
+          const auto low = __builtin_amdgcn_permlane32_swap(w[0][i], w[1][i], false, false);
+          const auto high = __builtin_amdgcn_permlane32_swap(w[2][i], w[3][i], false, false);
+          const auto even = __builtin_amdgcn_permlane16_swap(low[0], high[0], false, false);
+          const auto odd = __builtin_amdgcn_permlane16_swap(low[1], high[1], false, false);
+          first[i] = even[0], first[2 + i] = odd[0], second[i] = even[1], second[2 + i] = odd[1];
         }
-        __builtin_amdgcn_sched_barrier(0);  // one part's values at a time: more would not fit the registers
+        const int row = (2 * m + mw) * 32 + store_row;
+        const bool inside = column < columns;
+        __builtin_amdgcn_raw_buffer_store_b128(first, out, inside ? (row * columns + column) * 2 : kOutside, 0, kOutputPolicy);
+        __builtin_amdgcn_raw_buffer_store_b128(second, out, inside ? ((row + 16) * columns + column) * 2 : kOutside, 0, kOutputPolicy);
+        __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: more would not fit the registers
       }
     }
     idle_stores<(kMaxBlocks - kBlocks) * kStores / kMaxBlocks>(out);
