@@ -36,12 +36,23 @@ __device__ __forceinline__ Segment segment_of(const ExpertMatmulArgs& a, int e) 
 // 64 lanes x 16 bytes from global memory to 1 KiB of LDS at `lds` (wave-uniform), not waited for.  In
 // assembly because the compiler would wait for every load before the next LDS read of any address; the
 // waits are written at the end of each step instead.  A lane whose offset lies outside the descriptor moves
-// zeros and makes no memory request.
+// zeros and makes no memory request.  kStream (the streaming hint) is for weights that one tile of rows reads and
+// nobody again: they pass the memory-side cache by, which keeps the products until the next operator reads them, and
+// the memory does not turn round between reads and writes all the time.  256 experts of 64 rows x 4096 x 4096: 823 us with
+// neither this nor the results written through into that cache, 788 with the first only, 698 with both; where tiles share
+// their weights the hint costs (8192^3 435 us without, 474 with).
+template <bool kStream = false>
 __device__ __forceinline__ void load_to_lds(int4v descriptor, int lds, int lane_offset, int scalar_offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(lds), "v"(lane_offset), "s"(descriptor), "s"(scalar_offset)
-               : "memory");
+  if constexpr (kStream)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                 :
+                 : "s"(lds), "v"(lane_offset), "s"(descriptor), "s"(scalar_offset)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(lane_offset), "s"(descriptor), "s"(scalar_offset)
+                 : "memory");
 }
 __device__ __forceinline__ void load_word_to_lds(int4v descriptor, int lds, int lane_offset) {  // 4 bytes a lane
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
@@ -226,7 +237,10 @@ __host__ __device__ constexpr int stages_of(int blocks) { return blocks <= 2 ? 3
 static_assert(stages_of(1) * stage_bytes_of(1) <= kRingBytes && stages_of(2) * stage_bytes_of(2) <= kRingBytes &&
                   stages_of(3) * stage_bytes_of(3) <= kRingBytes && stages_of(4) * stage_bytes_of(4) <= kRingBytes,
               "the ring");
-constexpr int kOutputPolicy = kCachePolicyStreaming | kCachePolicyDeviceScope;
+// Results of up to this many bytes are written through into the 256 MB memory-side cache where the weights pass that cache
+// by (256 x 64 rows x 4096, 134 MB, k 4096: 698 us, streamed 737); more would push one another out (256 x 128 rows x 7168,
+// 470 MB, k 2048: 840, streamed 768), and so do weights that go through it (8192^3: 471, streamed 442).
+constexpr long long kCachedOutput = 192LL << 20;
 constexpr int kTableAt = kRingBytes;    // row tiles before every thread's experts
 constexpr int kRowScaleBytes = kMaxBlocks * kBlockRows * 4;
 constexpr int kScaleBytes = kRowScaleBytes + kBigN * 4;
@@ -241,6 +255,7 @@ __device__ __forceinline__ int row_tiles_of(int blocks) { return (blocks + kMaxB
 struct BigTile {
   int expert, column;  // first output column
   int first, rows;     // rows of a
+  int only;            // no other tile has rows of the expert
 };
 
 // One workgroup's walk over its tiles.  Wave (mw, nw) owns the 32-row blocks mw, mw + 2, ... and 128 of the 256
@@ -251,6 +266,7 @@ struct BigMatmul {
   const ExpertMatmulArgs& a;
   unsigned char* const lds;
   const int lds_base, lane, wave, mw, nw, K, columns, steps;
+  const bool stream_output;
   int4v desc_a, desc_b;
 
   // The same value, but not the same for the compiler: what is derived from it is computed where it is used
@@ -269,13 +285,15 @@ struct BigMatmul {
         nw(wave >> 1),
         K(args.in_features),
         columns(kSilu ? args.out_features / 2 : args.out_features),
-        steps((args.in_features + kStageK - 1) / kStageK) {}
+        steps((args.in_features + kStageK - 1) / kStageK),
+        stream_output(static_cast<long long>(args.num_rows) * columns > kCachedOutput / 2) {}
 
   // Load j of stage `step`, whose place in the ring is `slot`: eight rows of the channels, or of the tokens.
+  template <bool kOnce>
   __device__ __forceinline__ void load_b(const Place& at, int slot, int step, int j) const {
     const int row = (kSilu ? wave & 1 : wave) * 64 + at.row + j * 8, piece = at.piece_of(j);
-    load_to_lds(desc_b, lds_base + slot + (wave * 8 + j) * kChunkBytes,
-                step * kStageK + piece < K ? row * K + piece : kOutside, step * kStageK);
+    load_to_lds<kOnce>(desc_b, lds_base + slot + (wave * 8 + j) * kChunkBytes,
+                       step * kStageK + piece < K ? row * K + piece : kOutside, step * kStageK);
   }
   __device__ __forceinline__ void load_a(const Place& at, int slot, int step, int j) const {
     const int eight = (j >> 1) * 8 + wave * 2 + (j & 1), piece = at.piece_of(j);
@@ -301,8 +319,13 @@ struct BigMatmul {
     const int stages = stages_of(blocks);
     for (int s = 0; s < stages && s < steps; ++s) {
       const int slot = s * stage_bytes_of(blocks);
+      if (tile.only != 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) load_b(at, slot, s, j);
+        for (int j = 0; j < 8; ++j) load_b<true>(at, slot, s, j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load_b<false>(at, slot, s, j);
+      }
 #pragma unroll
       for (int j = 0; j < 2 * kMaxBlocks; ++j)
         if (j < 2 * blocks) load_a(at, slot, s, j);
@@ -329,7 +352,7 @@ struct BigMatmul {
   enum Loads { kNone, kChannels, kRows };
   // A quarter of a stage's products; between them, spread over them, the reads of the next quarter's fragments (from
   // the stage in `from`, or with kRead false none) and the loads of a part of stage `ahead` (to `to`).
-  template <int kBlocks, int kQuarter, Loads kLoad, bool kRead = true>
+  template <int kBlocks, bool kOnce, int kQuarter, Loads kLoad, bool kRead = true>
   __device__ __forceinline__ void quarter(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int from, int to,
                                           int ahead) const {
     constexpr int kLoads = kLoad == kNone ? 0 : kLoad == kChannels ? 8 : 2 * kBlocks;
@@ -340,7 +363,7 @@ struct BigMatmul {
       for (int i = p * kItems / kProducts; i < (p + 1) * kItems / kProducts; ++i) {
         const int loads_before = kLoads == 0 ? 0 : (i + 1) * kLoads / kItems;
         const bool is_load = kLoads != 0 && loads_before != i * kLoads / kItems;
-        if (is_load) kLoad == kChannels ? load_b(at, to, ahead, loads_before - 1) : load_a(at, to, ahead, loads_before - 1);
+        if (is_load) kLoad == kChannels ? load_b<kOnce>(at, to, ahead, loads_before - 1) : load_a(at, to, ahead, loads_before - 1);
         else read<kBlocks>(at, f, from, (kQuarter + 1) & 3, i - loads_before);
       }
       constexpr int h = kQuarter & 1;
@@ -351,7 +374,7 @@ struct BigMatmul {
 
   // The products of one tile whose rows fill kBlocks pairs of 32-row blocks, the start of the next tile, and
   // the epilogue.
-  template <int kBlocks>
+  template <int kBlocks, bool kOnce>
   __device__ __forceinline__ void run(const BigTile& tile, int scales_at, bool has_next, const BigTile& next, int next_scales_at) {
     const Place at(fresh(lane));
     int16v acc[kBlocks][4];
@@ -368,9 +391,9 @@ struct BigMatmul {
       wait_and_meet<kStores>();
 #pragma unroll
     for (int i = 0; i < 4 + kBlocks; ++i) read<kBlocks>(at, f, 0, 0, i);
-    quarter<kBlocks, 0, kNone>(at, f, acc, 0, 0, 0);
-    quarter<kBlocks, 1, kNone>(at, f, acc, 0, 0, 0);
-    quarter<kBlocks, 2, kNone>(at, f, acc, 0, 0, 0);
+    quarter<kBlocks, kOnce, 0, kNone>(at, f, acc, 0, 0, 0);
+    quarter<kBlocks, kOnce, 1, kNone>(at, f, acc, 0, 0, 0);
+    quarter<kBlocks, kOnce, 2, kNone>(at, f, acc, 0, 0, 0);
     // The barrier behind the third quarter of stage s makes stage s + 1 visible (younger ones and at first the previous
     // tile's stores may still be on their way), and tells that every wave has read all of stage s, whose place stage
     // s + kStages then fills.
@@ -379,10 +402,10 @@ struct BigMatmul {
     const auto go_on = [&](auto load) {
       constexpr bool kLoad = decltype(load)::value;
       const int next_slot = after(here), ahead = step + kStages;
-      quarter<kBlocks, 3, kLoad ? kChannels : kNone>(at, f, acc, next_slot, here, ahead);
-      quarter<kBlocks, 0, kLoad ? kRows : kNone>(at, f, acc, next_slot, here, ahead);
-      quarter<kBlocks, 1, kNone>(at, f, acc, next_slot, 0, 0);
-      quarter<kBlocks, 2, kNone>(at, f, acc, next_slot, 0, 0);
+      quarter<kBlocks, kOnce, 3, kLoad ? kChannels : kNone>(at, f, acc, next_slot, here, ahead);
+      quarter<kBlocks, kOnce, 0, kLoad ? kRows : kNone>(at, f, acc, next_slot, here, ahead);
+      quarter<kBlocks, kOnce, 1, kNone>(at, f, acc, next_slot, 0, 0);
+      quarter<kBlocks, kOnce, 2, kNone>(at, f, acc, next_slot, 0, 0);
       ++step;
       here = next_slot;
     };
@@ -400,7 +423,7 @@ struct BigMatmul {
       go_on(std::false_type{});
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    quarter<kBlocks, 3, kNone, false>(at, f, acc, 0, 0, 0);
+    quarter<kBlocks, kOnce, 3, kNone, false>(at, f, acc, 0, 0, 0);
     // The next tile's loads run during this one's epilogue.
     if (has_next) start(next, next_scales_at);
 
@@ -454,8 +477,15 @@ struct BigMatmul {
         }
         const int row = (2 * m + mw) * 32 + store_row;
         const bool inside = column < columns;
-        __builtin_amdgcn_raw_buffer_store_b128(first, out, inside ? (row * columns + column) * 2 : kOutside, 0, kOutputPolicy);
-        __builtin_amdgcn_raw_buffer_store_b128(second, out, inside ? ((row + 16) * columns + column) * 2 : kOutside, 0, kOutputPolicy);
+        const int at_first = inside ? (row * columns + column) * 2 : kOutside;
+        const int at_second = inside ? ((row + 16) * columns + column) * 2 : kOutside;
+        if (!kOnce || stream_output) {
+          __builtin_amdgcn_raw_buffer_store_b128(first, out, at_first, 0, kCachePolicyDeviceScope | kCachePolicyStreaming);
+          __builtin_amdgcn_raw_buffer_store_b128(second, out, at_second, 0, kCachePolicyDeviceScope | kCachePolicyStreaming);
+        } else {
+          __builtin_amdgcn_raw_buffer_store_b128(first, out, at_first, 0, kCachePolicyDeviceScope);
+          __builtin_amdgcn_raw_buffer_store_b128(second, out, at_second, 0, kCachePolicyDeviceScope);
+        }
         __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: more would not fit the registers
       }
     }
@@ -546,7 +576,7 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
     const int from = static_cast<int>(static_cast<long long>(row_tile) * blocks / row_tiles) * kBlockRows;
     const int to = static_cast<int>(static_cast<long long>(row_tile + 1) * blocks / row_tiles) * kBlockRows;
     return BigTile{expert, column_tile * kColumns, __builtin_amdgcn_readfirstlane(all.first) + from,
-                   (to < rows ? to : rows) - from};
+                   (to < rows ? to : rows) - from, row_tiles == 1 ? 1 : 0};
   };
 
   // Workgroups go to the eight dies in turn; each die takes one contiguous run of the tiles, so that the rows
@@ -573,11 +603,17 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
     const bool has_next = index < end;
     const BigTile next = has_next ? locate(index) : tile;
     const int at = scales_at + turn * kScaleBytes, next_at = scales_at + (turn ^ 1) * kScaleBytes;
-    switch ((tile.rows + kBlockRows - 1) / kBlockRows) {
-      case 1: matmul.template run<1>(tile, at, has_next, next, next_at); break;
-      case 2: matmul.template run<2>(tile, at, has_next, next, next_at); break;
-      case 3: matmul.template run<3>(tile, at, has_next, next, next_at); break;
-      default: matmul.template run<4>(tile, at, has_next, next, next_at); break;
+    const int blocks = (tile.rows + kBlockRows - 1) / kBlockRows;
+    if (tile.only != 0) switch (blocks) {
+      case 1: matmul.template run<1, true>(tile, at, has_next, next, next_at); break;
+      case 2: matmul.template run<2, true>(tile, at, has_next, next, next_at); break;
+      case 3: matmul.template run<3, true>(tile, at, has_next, next, next_at); break;
+      default: matmul.template run<4, true>(tile, at, has_next, next, next_at); break;
+    }
+    else switch (blocks) {  // the shares of at least five blocks
+      case 2: matmul.template run<2, false>(tile, at, has_next, next, next_at); break;
+      case 3: matmul.template run<3, false>(tile, at, has_next, next, next_at); break;
+      default: matmul.template run<4, false>(tile, at, has_next, next, next_at); break;
     }
     if (!has_next) return;
     tile = next;
