@@ -49,14 +49,14 @@ __device__ __forceinline__ bf16x8 as_bf16(vec16 v) {
 }
 
 // A chunk is 128 contiguous bytes of 16 weight rows, whole cache lines, in two 16-byte loads of a lane: lane l has
-// row l % 16 and the l / 16-th 32 bytes.  The columns' vectors are read in the same order over k, which is all a
-// product needs.
+// row l % 16 and the l / 16-th 16 bytes of either half.  The columns' vectors are read in the same order over k, which
+// is all a product needs.
 template <bool kInt8>
 struct Chunk {
   static constexpr int kBytes = kInt8 ? 1 : 2;
   static constexpr int kPiece = 16 / kBytes;      // elements of a load of weights
-  static constexpr int kLane = 2 * kPiece;        // of a lane
-  static constexpr int kElements = 4 * kLane;     // of k
+  static constexpr int kHalf = 4 * kPiece;        // of the four lanes of a row
+  static constexpr int kElements = 2 * kHalf;     // of k
   static constexpr int kVectors = kInt8 ? 2 : 1;  // 16-byte bf16 loads of a column for a load of weights
   static constexpr int kAll = 2 * kVectors;       // and for a lane's whole chunk
 };
@@ -171,8 +171,8 @@ struct Stream {
   __device__ __forceinline__ void load(int slot, __amdgpu_buffer_rsrc_t vectors) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const bool inside = k + h * C::kPiece < k_end;
-      const int at = inside ? w_lane + k * C::kBytes + h * 16 : kOutside;
+      const bool inside = k + h * C::kHalf < k_end;
+      const int at = inside ? w_lane + (k + h * C::kHalf) * C::kBytes : kOutside;
 #pragma unroll
       for (int m = 0; m < kMatrices; ++m)
         w[slot][h][m] = __builtin_amdgcn_raw_buffer_load_b128(rows_of(rows[m], row_bytes), at, 0, 0);
@@ -180,10 +180,11 @@ struct Stream {
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
       const int v = l * kFold + (kFold > 1 ? lane_fold() : 0);
-      const bool inside = k + v / C::kVectors * C::kPiece < k_end;
+      const int at = k + v / C::kVectors * C::kHalf + v % C::kVectors * 8;
+      const bool inside = at < k_end;
 #pragma unroll
       for (int c = 0; c < kBlocks; ++c)
-        x[slot][c][l] = __builtin_amdgcn_raw_buffer_load_b128(vectors, inside ? x_at[c] + k * 2 + v * 16 : kOutside, 0, 0);
+        x[slot][c][l] = __builtin_amdgcn_raw_buffer_load_b128(vectors, inside ? x_at[c] + at * 2 : kOutside, 0, 0);
     }
     k += C::kElements;
   }
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
   const int chunks = (H + C::kElements - 1) / C::kElements;
   const int share = (chunks + kFirstWaves - 1) / kFirstWaves;  // of a wave
   const int rounds = (share + kDepth - 1) / kDepth;
-  const int k_lane = (lane >> 4) * C::kLane;
+  const int k_lane = (lane >> 4) * C::kPiece;
   const int k_begin = share * wave * C::kElements + k_lane;
   const int share_end = share * (wave + 1) * C::kElements;
   const int k_stop = share_end < H ? share_end : H;
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(c
   const int chunks = (I + C::kElements - 1) / C::kElements;
   const int share = (chunks + splits - 1) / splits;
   const int rounds = (share + kDepth - 1) / kDepth;
-  const int k_lane = (lane >> 4) * C::kLane;
+  const int k_lane = (lane >> 4) * C::kPiece;
 
   const __amdgpu_buffer_rsrc_t vectors = rows_of(a.act, routes * I * 4);
   S s;
