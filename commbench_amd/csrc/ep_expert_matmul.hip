@@ -18,6 +18,7 @@ constexpr int kChunkBytes = 1024;                              // what one load 
 constexpr int kOutside = static_cast<int>(0x80000000u);        // an offset beyond every descriptor
 
 typedef int int16v __attribute__((ext_vector_type(16)));
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
 
 struct Segment {
   int first, rows;
@@ -96,19 +97,20 @@ constexpr int kSmallThreads = 256;
 
 struct RowTile {
   int expert, first, rows;  // rows [first, first + rows) of a and out; rows == 0: no such tile
+  int only;                 // no other tile has rows of the expert
 };
 
 // The `index`-th tile of up to kTileM rows, the experts' segments cut into tiles one after the other.
 __device__ __forceinline__ RowTile find_row_tile(const ExpertMatmulArgs& a, int index) {
   if (a.expert_offsets == nullptr) {
     const int left = a.num_rows - index * kTileM;
-    return RowTile{0, index * kTileM, left < 0 ? 0 : left < kTileM ? left : kTileM};
+    return RowTile{0, index * kTileM, left < 0 ? 0 : left < kTileM ? left : kTileM, a.num_rows <= kTileM ? 1 : 0};
   }
   __shared__ int wave_tiles[kSmallThreads / kWave];
   __shared__ RowTile found;
   const int t = static_cast<int>(threadIdx.x);
   const int per = (a.num_experts + kSmallThreads - 1) / kSmallThreads;
-  if (t == 0) found = RowTile{0, 0, 0};
+  if (t == 0) found = RowTile{0, 0, 0, 0};
   Segment segments[kMaxExperts / kSmallThreads];
   int mine = 0;
 #pragma unroll
@@ -128,13 +130,13 @@ __device__ __forceinline__ RowTile find_row_tile(const ExpertMatmulArgs& a, int 
     if (index >= before && index < before + tiles) {
       const int skip = (index - before) * kTileM;
       found = RowTile{t * per + j, segments[j].first + skip,
-                      segments[j].rows - skip < kTileM ? segments[j].rows - skip : kTileM};
+                      segments[j].rows - skip < kTileM ? segments[j].rows - skip : kTileM, tiles == 1 ? 1 : 0};
     }
     before += tiles;
   }
   __syncthreads();
   return RowTile{__builtin_amdgcn_readfirstlane(found.expert), __builtin_amdgcn_readfirstlane(found.first),
-                 __builtin_amdgcn_readfirstlane(found.rows)};
+                 __builtin_amdgcn_readfirstlane(found.rows), __builtin_amdgcn_readfirstlane(found.only)};
 }
 
 // Wave (mw, nw) owns 32 rows and 32 columns (with kSilu their gate and their up channels).
@@ -162,50 +164,56 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
   const int4v desc_up = kSilu ? descriptor_of(a.b + (channel + columns) * K, b_rows * K) : desc_b;
   const int offset = (wave * 16 + at.row) * K;
   const int ring_base = lds_address(ring);
-  int load_slot = 0;
-  const auto load_stage = [&](int step) {  // steps behind the last load nothing, but count
-    const int k0 = step < steps ? step * kStageK : 0;
-    const int to = ring_base + load_slot * kStage + wave * 2 * kChunkBytes;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int piece = at.piece_of(j);
-      const int from = step * kStageK + piece < K ? offset + j * 8 * K + piece : kOutside;
-      load_to_lds(desc_a, to + j * kChunkBytes, from, k0);
-      load_to_lds(desc_b, to + kABytes + j * kChunkBytes, from, k0);
-      if constexpr (kSilu) load_to_lds(desc_up, to + kABytes + kTileN * kStageK + j * kChunkBytes, from, k0);
-    }
-    load_slot = load_slot + 1 == kRing ? 0 : load_slot + 1;
-  };
-#pragma unroll
-  for (int s = 0; s < kRing - 1; ++s) load_stage(s);
-
   int16v acc[kSets];
 #pragma unroll
   for (int s = 0; s < kSets; ++s) acc[s] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-  int slot = 0;
-  for (int step = 0; step < steps; ++step) {
-    // Stage step is in, and every wave has left the stage before it, whose place the next load takes.
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((kRing - 2) * kLoads) : "memory");
-    load_stage(step + kRing - 1);
-    const unsigned char* stage = ring + slot * kStage;
+  const auto products = [&](auto once) {
+    constexpr bool kOnce = decltype(once)::value;
+    int load_slot = 0;
+    const auto load_stage = [&](int step) {  // steps behind the last load nothing, but count
+      const int k0 = step < steps ? step * kStageK : 0;
+      const int to = ring_base + load_slot * kStage + wave * 2 * kChunkBytes;
 #pragma unroll
-    for (int quarter = 0; quarter < 4; ++quarter) {
-      const unsigned char* base = stage + (at.read_at ^ (quarter * 32));
-      const int4v rows = *reinterpret_cast<const int4v*>(base + mw * 32 * kStageK);
-#pragma unroll
-      for (int s = 0; s < kSets; ++s) {
-        const int4v channels = *reinterpret_cast<const int4v*>(base + kABytes + (s * kTileN + nw * 32) * kStageK);
-        acc[s] = __builtin_amdgcn_mfma_i32_32x32x32_i8(channels, rows, acc[s], 0, 0, 0);
+      for (int j = 0; j < 2; ++j) {
+        const int piece = at.piece_of(j);
+        const int from = step * kStageK + piece < K ? offset + j * 8 * K + piece : kOutside;
+        load_to_lds(desc_a, to + j * kChunkBytes, from, k0);
+        load_to_lds<kOnce>(desc_b, to + kABytes + j * kChunkBytes, from, k0);
+        if constexpr (kSilu) load_to_lds<kOnce>(desc_up, to + kABytes + kTileN * kStageK + j * kChunkBytes, from, k0);
       }
+      load_slot = load_slot + 1 == kRing ? 0 : load_slot + 1;
+    };
+#pragma unroll
+    for (int s = 0; s < kRing - 1; ++s) load_stage(s);
+    int slot = 0;
+    for (int step = 0; step < steps; ++step) {
+      // Stage step is in, and every wave has left the stage before it, whose place the next load takes.
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((kRing - 2) * kLoads) : "memory");
+      load_stage(step + kRing - 1);
+      const unsigned char* stage = ring + slot * kStage;
+#pragma unroll
+      for (int quarter = 0; quarter < 4; ++quarter) {
+        const unsigned char* base = stage + (at.read_at ^ (quarter * 32));
+        const int4v rows = *reinterpret_cast<const int4v*>(base + mw * 32 * kStageK);
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const int4v channels = *reinterpret_cast<const int4v*>(base + kABytes + (s * kTileN + nw * 32) * kStageK);
+          acc[s] = __builtin_amdgcn_mfma_i32_32x32x32_i8(channels, rows, acc[s], 0, 0, 0);
+        }
+      }
+      slot = slot + 1 == kRing ? 0 : slot + 1;
     }
-    slot = slot + 1 == kRing ? 0 : slot + 1;
-  }
+  };
+  if (tile.only != 0) products(std::true_type{});
+  else products(std::false_type{});
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the workgroup's LDS
 
   // Lane l holds row l % 32 and channels 8 g + 4 (l / 32) + 0..3.
   const int row = mw * 32 + r;
   if (row >= tile.rows) return;
   const float row_scale = a.a_scales[static_cast<size_t>(tile.first + row) * a.a_scales_row_stride];
+  const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(a.out + static_cast<size_t>(tile.first) * columns, 0,
+                                                                       tile.rows * columns * 2, kRawBufferFormat);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int n = n0 + nw * 32 + g * 8 + (lane >> 5) * 4;
@@ -217,8 +225,8 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
       o[i] = static_cast<float>(acc[0][g * 4 + i]) * (row_scale * scales[i]);
       if constexpr (kSilu) o[i] = silu(o[i]) * (static_cast<float>(acc[kSets - 1][g * 4 + i]) * (row_scale * scales[columns + i]));
     }
-    *reinterpret_cast<uint2*>(a.out + static_cast<size_t>(tile.first + row) * columns + n) =
-        uint2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])};
+    __builtin_amdgcn_raw_buffer_store_b64(words2{to_bf16_pair(o[0], o[1]), to_bf16_pair(o[2], o[3])}, out,
+                                          (row * columns + n) * 2, 0, kCachePolicyDeviceScope);
   }
 }
 
