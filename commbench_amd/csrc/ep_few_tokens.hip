@@ -12,16 +12,17 @@
 #include <atomic>
 
 #include "ep_device.h"
+#include "ep_stage.h"
 
 namespace mi_ep {
 namespace {
 
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kFirstThreads = 256, kFirstWaves = kFirstThreads / kWave;
 constexpr int kSecondThreads = 512, kSecondWaves = kSecondThreads / kWave;
-constexpr int kOutside = static_cast<int>(0x80000000u);  // an offset beyond every descriptor: the load returns zeros
 
 // 8 of the int8 codes in two words as bf16 (every code is one exactly).
 __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
@@ -65,6 +66,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int 
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, kRawBufferFormat);
 }
 __device__ __forceinline__ void wait_lds_and_meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// silu(g) * u as the sum of two bf16 values.
+__device__ __forceinline__ void activate(float g, float u, uint32_t& high, uint32_t& low) {
+  const float act = g / (1.0f + __expf(-g)) * u;
+  high = f32_to_bf16_bits(act);
+  low = __builtin_isfinite(act) ? f32_to_bf16_bits(act - bf16_lo(high)) : 0;  // the rest of an infinity is none
+}
 
 // Who meets whom, made by every workgroup for itself from the ids: `entries` lists the met experts by their
 // first routes, once for every kPass of an expert's routes (first route | pass << 10).
@@ -330,18 +338,166 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
           g *= scales[0];
           u *= scales[I];
         }
-        const float act = g / (1.0f + __expf(-g)) * u;
-        const uint32_t high = f32_to_bf16_bits(act);
+        uint32_t high, low;
+        activate(g, u, high, low);
         uint16_t* out = a.act + static_cast<size_t>(column_route) * I + i0 + n;
         out[0] = static_cast<uint16_t>(high);
-        // The rest of an infinity is none.
-        const float rest = act - bf16_lo(high);
-        out[static_cast<size_t>(routes) * I] = __builtin_isfinite(act) ? static_cast<uint16_t>(f32_to_bf16_bits(rest)) : 0;
+        out[static_cast<size_t>(routes) * I] = static_cast<uint16_t>(low);
       }
     }
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) route[c] = next_route[c];
   }
+}
+
+// Gate and up where there are many (entry, 64 columns of act) items: workgroup b takes the b-th contiguous share of them.
+// Wave w owns channels 16 w .. 16 w + 15 of an item's gate and up rows.  A stage is 128 bytes of k of the 128 weight rows
+// and the entry's vectors over the same k; it comes by loads of whole lines past the registers and past the memory-side
+// cache, which is what the memory delivers fastest.  The stages of an item and of the next run on in one ring of three.
+constexpr int kSliceColumns = 64, kTileRing = 3;
+constexpr int kTileVectorsAt = 2 * kSliceColumns * kStageK;            // 16 vectors behind the weights, 1 KiB for four of them
+constexpr int kTileStage = kTileVectorsAt + 4 * kChunkBytes;
+constexpr int kTileScalesAt = kTileRing * kTileStage;                  // two items' scales, 256 bytes a wave
+constexpr int kTileMeetingAt = kTileScalesAt + 2 * kFirstWaves * 256;
+static_assert(kTileScalesAt >= 2 * kMaxExperts * static_cast<int>(sizeof(int)), "scratch of the meeting");
+
+template <bool kInt8>
+__global__ __launch_bounds__(kFirstThreads, 2) void ep_few_tokens_gate_up_tiles_kernel(const FewTokensArgs a) {
+  constexpr int kBytes = kInt8 ? 1 : 2;
+  constexpr int kElements = kStageK / kBytes;      // of k in a stage
+  constexpr int kVectorBytes = 2 * kElements;      // of a column in a stage
+  constexpr int kPieces = kVectorBytes / 16;       // 16 (int8 weights) or 8
+  constexpr int kLoads = 5, kStores = 2;           // of a wave: for a stage, for an item's results
+  extern __shared__ __align__(1024) unsigned char lds[];
+  __shared__ uint16_t lists[kFirstWaves][16];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int routes = a.num_tokens * a.num_topk;
+  Meeting<16> meeting;
+  meeting.make(a, routes, lds + kTileMeetingAt, reinterpret_cast<int*>(lds));
+
+  const int H = a.hidden, I = a.intermediate;
+  const int slices = (I + kSliceColumns - 1) / kSliceColumns;
+  const long long items = static_cast<long long>(meeting.count) * slices, workgroups = static_cast<long long>(gridDim.x);
+  const int from = static_cast<int>(items * blockIdx.x / workgroups), to = static_cast<int>(items * (blockIdx.x + 1) / workgroups);
+  if (from >= to) return;
+  const int steps = (H + kElements - 1) / kElements;
+  const Place at(lane);
+  const int lds_base = lds_address(lds);
+
+  // Vectors: a load of wave w fills columns 4 w .. 4 w + 3; their pieces are permuted so that 16 lanes that read one piece of
+  // the 16 columns meet all banks.  Lane l multiplies column l % 16.
+  const int load_lane = lane & (4 * kPieces - 1);
+  const int load_column = wave * 4 + load_lane / kPieces;
+  const int load_piece = (load_lane & (kPieces - 1)) ^ (kInt8 ? load_column : load_column >> 1);
+  const int read_column = lane & 15;
+  const int read_vector = kTileVectorsAt + (read_column >> 2) * kChunkBytes + (read_column & 3) * kVectorBytes;
+  const int column[2] = {read_column, load_column};
+  const int4v desc_x = descriptor_of(a.x, a.num_tokens * H * 2);
+
+  int ahead = from, ahead_step = 0, ahead_entry = -1, ahead_slot = 0;  // where the loads stand
+  int next_route[2] = {-1, -1}, route = -1, next_item_route = -1, vector_at = kOutside;
+  int4v desc_gate = desc_x, desc_up = desc_x;
+  const auto load_stage = [&]() {
+    if (ahead_step == 0 && ahead < to) {
+      const int entry = ahead / slices, e = meeting.expert(entry), i0 = (ahead - entry * slices) * kSliceColumns;
+      if (entry != ahead_entry) {
+        meeting.template columns<2>(entry, routes, lists[wave], column, next_route);
+        vector_at = next_route[1] >= 0 && load_lane == lane ? next_route[1] / a.num_topk * H * 2 : kOutside;
+        ahead_entry = entry;
+      }
+      next_item_route = next_route[0];
+      const int rows = I - i0 < kSliceColumns ? I - i0 : kSliceColumns;
+      const unsigned char* gate = a.w13 + (static_cast<size_t>(e) * 2 * I + i0) * H * kBytes;
+      desc_gate = descriptor_of(gate, rows * H * kBytes);
+      desc_up = descriptor_of(gate + static_cast<size_t>(I) * H * kBytes, rows * H * kBytes);
+      if constexpr (kInt8) {  // lanes 0 to 15: the wave's gate scales, 16 to 31: its up scales
+        const float* scales = a.w13_scales + static_cast<size_t>(e) * 2 * I;
+        const int row = i0 + wave * 16 + (lane & 15);
+        load_word_to_lds(descriptor_of(scales, 2 * I * 4), lds_base + kTileScalesAt + ((ahead & 1) * kFirstWaves + wave) * 256,
+                         lane < 32 && row < I ? (row + (lane >> 4) * I) * 4 : kOutside);
+      }
+    }
+    const int k0 = ahead_step * kStageK;
+    const int to_slot = lds_base + ahead_slot * kTileStage;
+    const bool live = ahead < to;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int piece = at.piece_of(j);
+      const int offset = live && k0 + piece < H * kBytes ? (wave * 16 + j * 8 + at.row) * H * kBytes + piece : kOutside;
+      load_to_lds<true>(desc_gate, to_slot + (wave * 2 + j) * kChunkBytes, offset, k0);
+      load_to_lds<true>(desc_up, to_slot + (8 + wave * 2 + j) * kChunkBytes, offset, k0);
+    }
+    const int k = ahead_step * kVectorBytes;
+    load_to_lds(desc_x, to_slot + kTileVectorsAt + wave * kChunkBytes,
+                live && vector_at >= 0 && k + load_piece * 16 < H * 2 ? vector_at + load_piece * 16 : kOutside, k);
+    ahead_slot = ahead_slot + 1 == kTileRing ? 0 : ahead_slot + 1;
+    if (++ahead_step == steps) {
+      ahead_step = 0;
+      ++ahead;
+    }
+  };
+  const __amdgpu_buffer_rsrc_t act = rows_of(a.act, routes * I * 4);
+
+#pragma unroll
+  for (int s = 0; s < kTileRing - 1; ++s) load_stage();
+  int slot = 0, since = kTileRing;  // stages since the last results were stored
+  for (int item = from; item < to; ++item) {
+    // At the start of an item the loads are two stages ahead, still in this item: it has two stages at least.
+    float4v gate = {0, 0, 0, 0}, up = {0, 0, 0, 0};
+    for (int step = 0; step < steps; ++step) {
+      // This stage is in (the next one and an item's stores may be on their way), and every wave has left the stage before
+      // it, whose place the next load takes.
+      if (since < kTileRing - 1)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((kTileRing - 2) * kLoads + kStores) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((kTileRing - 2) * kLoads) : "memory");
+      ++since;
+      if (step == 0) route = next_item_route;
+      load_stage();
+      const unsigned char* stage = lds + slot * kTileStage;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // Rows are permuted by half their number, as Place says.
+        const int piece = ((h * 4 + (lane >> 4)) ^ ((read_column >> 1) & 7)) * 16;
+        const vec16 g = *reinterpret_cast<const vec16*>(stage + (wave * 16 + read_column) * kStageK + piece);
+        const vec16 u = *reinterpret_cast<const vec16*>(stage + (kSliceColumns + wave * 16 + read_column) * kStageK + piece);
+        if constexpr (kInt8) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int of = (((h * 4 + (lane >> 4)) * 2 + i) ^ read_column) * 16;
+            const bf16x8 x = as_bf16(*reinterpret_cast<const vec16*>(stage + read_vector + of));
+            gate = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(g[2 * i], g[2 * i + 1]), x, gate, 0, 0, 0);
+            up = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(u[2 * i], u[2 * i + 1]), x, up, 0, 0, 0);
+          }
+        } else {
+          const int of = ((h * 4 + (lane >> 4)) ^ (read_column >> 1)) * 16;
+          const bf16x8 x = as_bf16(*reinterpret_cast<const vec16*>(stage + read_vector + of));
+          gate = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(g), x, gate, 0, 0, 0);
+          up = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(u), x, up, 0, 0, 0);
+        }
+      }
+      slot = slot + 1 == kTileRing ? 0 : slot + 1;
+    }
+    // Lane l holds channels 4 (l / 16) + 0..3 of column l % 16.
+    const int first = item % slices * kSliceColumns + wave * 16 + (lane >> 4) * 4;
+    if constexpr (kInt8) {
+      const float* scales = reinterpret_cast<const float*>(lds + kTileScalesAt + ((item & 1) * kFirstWaves + wave) * 256);
+      const float4 of_gate = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 4);
+      const float4 of_up = *reinterpret_cast<const float4*>(scales + 16 + (lane >> 4) * 4);
+      gate[0] *= of_gate.x, gate[1] *= of_gate.y, gate[2] *= of_gate.z, gate[3] *= of_gate.w;
+      up[0] *= of_up.x, up[1] *= of_up.y, up[2] *= of_up.z, up[3] *= of_up.w;
+    }
+    uint32_t high[4], low[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) activate(gate[i], up[i], high[i], low[i]);
+    const int offset = route >= 0 && first < I ? (route * I + first) * 2 : kOutside;
+    __builtin_amdgcn_raw_buffer_store_b64(words2{high[0] | high[1] << 16, high[2] | high[3] << 16}, act, offset, 0,
+                                          kCachePolicyDeviceScope);
+    __builtin_amdgcn_raw_buffer_store_b64(words2{low[0] | low[1] << 16, low[2] | low[3] << 16}, act, offset,
+                                          routes * I * 2, kCachePolicyDeviceScope);
+    since = 0;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the workgroup's LDS
 }
 
 // Down.  Workgroup h: 16 columns of the output for every token.  Items are the entries (with fewer of them than
@@ -465,6 +621,27 @@ hipError_t launch_gate_up(const FewTokensArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <bool kInt8>
+hipError_t launch_gate_up_tiles(const FewTokensArgs& a, int compute_units, hipStream_t stream) {
+  const int lds = kTileMeetingAt + static_cast<int>(Meeting<16>::bytes(a.num_tokens * a.num_topk));
+  int ordinal = 0;
+  hipError_t e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
+  if (e != hipSuccess) return e;
+  // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> lds_limit_raised[kMaxDevices];
+  if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
+  if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_gate_up_tiles_kernel<kInt8>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+    if (e != hipSuccess) return e;
+    lds_limit_raised[ordinal].store(1, std::memory_order_release);
+  }
+  hipLaunchKernelGGL((ep_few_tokens_gate_up_tiles_kernel<kInt8>), dim3(static_cast<unsigned>(2 * compute_units)),
+                     dim3(kFirstThreads), lds, stream, a);
+  return hipGetLastError();
+}
+
 template <bool kInt8, int kBlocks, int kDepth, int kFold>
 hipError_t launch_down(const FewTokensArgs& a, hipStream_t stream) {
   const int routes = a.num_tokens * a.num_topk;
@@ -497,7 +674,17 @@ hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
   // Columns of a pass by the routes that an expert gets on average: every further pass reads its weights again.
   const int routes = a.num_tokens * a.num_topk;
   const bool many = routes > 8 * a.num_experts;
-  const hipError_t e = many ? launch_gate_up<kInt8, 4, 1>(a, stream) : launch_gate_up<kInt8, 1, 2>(a, stream);
+  DeviceTraits dev{};
+  hipError_t e = device_traits(stream, &dev);
+  if (e != hipSuccess) return e;
+  // Tiles where every workgroup gets two items or more, on (at most) so many experts.  Without / with tiles in us: 48 tokens
+  // of top 8 over 256 experts, 7168 x 2048 int8 1564 / 1412; 16 over 128, 4096 x 1408 bf16 580 / 531; 4 tokens of the first
+  // (1024 items) 271 / 243, one token (256) 76 / 81; 12 tokens of top 4 over 64 experts, 4096 x 1024 (768) 116 / 128.
+  const long long met = routes < a.num_experts ? routes : a.num_experts;
+  const long long items = met * ((a.intermediate + kSliceColumns - 1) / kSliceColumns);
+  const bool tiles = !many && a.hidden > kStageK && items >= 4LL * dev.compute_units;
+  e = many ? launch_gate_up<kInt8, 4, 1>(a, stream)
+      : tiles ? launch_gate_up_tiles<kInt8>(a, dev.compute_units, stream) : launch_gate_up<kInt8, 1, 2>(a, stream);
   if (e != hipSuccess) return e;
   if (many) return launch_down<kInt8, 4, 1, 1>(a, stream);
   if (routes > 2 * a.num_experts) return launch_down<kInt8, 1, 4, 1>(a, stream);

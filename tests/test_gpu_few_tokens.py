@@ -65,6 +65,25 @@ FOLDS = [  # few routes for each expert, several for one of them; many for one, 
     (40, 64, 4, 160, 64, 0.0, "zipf"), (40, 64, 4, 528, 144, 0.2, "zipf"), (128, 1024, 8, 32, 16, 0.0, "uniform")]
 
 
+TILES = [  # enough experts and columns for the tiles of the first product: two stages and more, ragged columns, several passes
+    (128, 1024, 8, 144, 48, 0.0, "uniform"), (128, 1024, 8, 272, 64, 0.1, "zipf"), (64, 512, 4, 400, 272, 0.0, "uniform"),
+    (40, 512, 8, 256, 208, 0.3, "uniform"), (128, 300, 8, 160, 224, 0.05, "zipf"), (16, 256, 8, 1040, 528, 0.0, "uniform")]
+
+
+@pytest.mark.parametrize("T,E,K,H,I,mask,kind", TILES)
+@pytest.mark.parametrize("quantised", [True, False])
+def test_many_items_of_the_first_product(T, E, K, H, I, mask, kind, quantised):
+    print(f"tokens {T} experts {E} slots {K} hidden {H} intermediate {I} masked {mask} {kind} int8 {quantised}", flush=True)
+    assert min(T * K, E) * ((I + 63) // 64) >= 4 * 256
+    p = problem(T * 7 + H, T, E, K, H, I, quantised, mask, kind)
+    want, bound = reference(p)
+    g = on_gpu(p)
+    out = call(g)
+    xu.check_within(xu.f64(out), want, bound)
+    for _ in range(3):
+        assert torch.equal(call(g), out)
+
+
 @pytest.mark.parametrize("T,E,K,H,I,mask,kind", FOLDS)
 @pytest.mark.parametrize("quantised", [True, False])
 def test_experts_of_uneven_counts(T, E, K, H, I, mask, kind, quantised):
