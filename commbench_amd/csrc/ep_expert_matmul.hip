@@ -2,7 +2,14 @@
 // channel, for gfx950:
 //   c[m, n] = a_scale[m] * b_scale[e, n] * sum_k a[m, k] * b[e, n, k]     rows m of expert e's segment
 //   out = bf16(c)   or, gate and up in one product,   out[m, i] = bf16(silu(c[m, i]) * c[m, I + i])
-// The sum over k is exact in 32-bit integers (|a|, |b| <= 128 and k < 2^17).
+// The sum over k is exact in 32-bit integers (|a|, |b| <= 128 and k < 2^17); the scales, silu and the product are fp32,
+// rounded to bf16 once.  silu(gate) * up is formed where both sums lie in one lane, so the 2 I columns never reach memory.
+//
+// What bounds it depends on the rows of an expert.  Few rows: reading the weights once (256 experts x 4096 x 7168 with 2 rows
+// each 1071 us, 7.0 TB/s; with 32 rows 1126).  Hundreds: the matrix units at the clock that the card's power limit leaves
+// them (8192^3 442 us, 2490 TOP/s, clock near 1.6 GHz), less what ragged heights leave empty: a segment is computed in
+// blocks of 64 rows (8192 tokens' 65536 rows over 256 experts x 4096 x 7168: 2570 us, of which the empty part of the
+// blocks is an eighth).
 #include <atomic>
 #include <type_traits>
 
@@ -32,7 +39,9 @@ __device__ __forceinline__ Segment segment_of(const ExpertMatmulArgs& a, int e) 
 // v / (1 + exp(-v)); the reciprocal instruction is off by one unit in the last place at most.
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 
-// ---- small tiles: 64 rows by 64 columns, for problems of few tiles --------------------------------------
+// ---- small tiles: 64 rows by 64 columns, for problems of few tiles or of a few rows an expert -------------
+// A workgroup a tile, so that little work still spreads over the card (8 experts x 32 rows x 512 x 256: 5.4 us) and two or
+// three workgroups of a compute unit hide one another's start; a ring of three stages each.
 constexpr int kTileM = 64, kTileN = 64;
 constexpr int kSmallThreads = 256;
 
@@ -171,7 +180,13 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
   }
 }
 
-// ---- large tiles ------------------------------------------------------------------------------------
+// ---- large tiles: up to 256 rows by 256 channels ----------------------------------------------------------
+// One persistent workgroup a compute unit, four waves of 128 x 128: a stage's 64 KiB give 128 products of 32 x 32 x 32, half
+// a fragment read from LDS for each, and the accumulators fill the 256 registers that the products can add to directly.
+// With loads of 128 bytes a row (64: a sixth slower), LDS rows permuted so that no bank is met twice, reads and loads spread
+// between the products one by one, and the next tile's loads and this tile's stores on their way at once.
+// Rejected: 320-row tiles (the accumulators no longer fit beside the fragments and are copied about), tiles claimed from
+// counters (skewed routing 4 % slower, even routing 2 % faster), dies' runs cut by cost instead of by tiles (no gain).
 constexpr int kBigN = 256;       // channels of a tile: with kSilu 128 gate channels and their 128 up channels
 constexpr int kBlockRows = 64;   // a tile's rows come in pairs of 32-row blocks, one for each half of the waves
 constexpr int kMaxBlocks = 4;    // 256 rows: the accumulators fill the matrix units' own registers
@@ -576,9 +591,9 @@ hipError_t launch_expert_matmul(const ExpertMatmulArgs& a, hipStream_t stream) {
   if (a.num_rows == 0) return hipSuccess;
   const int columns = a.silu_mul ? a.out_features / 2 : a.out_features;
   // Large tiles where there are enough of them for most compute units and enough rows in each to be worth the
-  // accumulators.  Small / large in us: 256 experts x 4096 x 7168 with 2, 8, 16, 64 rows each: 1276 / 1314, 1307 / 1325,
-  // 1354 / 1341, 1565 / 1459; 64 large tiles (8 x 256 rows x 2048 channels, k 2048): 22 / 31, 128 of them (8 x 256 x
-  // 4096): 55 / 41, 104 (8 x 384 x 2048, k 4096): 73 / 58.
+  // accumulators.  Small / large in us: 256 experts x 4096 x 7168 with 4, 8, 16, 32 rows each: 1127 / 1128, 1145 / 1135,
+  // 1128 / 1099, 1232 / 1181; 64 large tiles (8 x 256 rows x 2048 channels, k 2048): 31 / 31, (1024 rows x 4096, k 4096):
+  // 36 / 44; 96 (8 x 384 x 2048, k 2048): 44 / 31; 128 (8 x 256 x 4096, k 2048): 57 / 35.
   const long long big_columns = a.silu_mul ? kBigN / 2 : kBigN;
   const long long by_rows = a.num_rows / (kMaxBlocks * kBlockRows);
   const long long by_experts = a.num_rows / 12 < a.num_experts ? a.num_rows / 12 : a.num_experts;
