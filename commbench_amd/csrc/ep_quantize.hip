@@ -63,6 +63,18 @@ struct Divisor {
   }
 };
 
+// Codes on their way to the expert's next product: written through into the memory-side cache (65536 x 2048 and read back:
+// 133.9 us left to the L2s, 131.3; 16384 x 2048 e4m3: 37.9 and 36.3).  The norm's, which are a small part of what it
+// writes, are left to the L2s (4096 x 4096: 32.3 us, written through 33.2).
+template <bool kNorm>
+__device__ __forceinline__ void store_codes(uint2* to, uint2 codes) {
+  if constexpr (kNorm)
+    *to = codes;
+  else
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), static_cast<uint64_t>(codes.y) << 32 | codes.x, __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // The scale of values whose largest magnitude has these bits.  Infinities and NaN order above every
 // finite value as integers, so a row (block) that holds one gets a NaN scale and reads back as NaN
 // throughout instead of as something finite.
@@ -215,7 +227,7 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       const int v = t + u * kRowThreads;
-      if (v < a.row_vecs) q[v] = quantize8<kFormat>(y[u], divide);
+      if (v < a.row_vecs) store_codes<kNorm>(q + v, quantize8<kFormat>(y[u], divide));
     }
   } else {
 #pragma unroll
@@ -224,7 +236,7 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
       const float scale = scale_of<kFormat>(block_max(amax[u]));  // every lane takes part
       if (v < a.row_vecs) {
         if (v % kQuantBlockLanes == 0) scales[static_cast<size_t>(v / kQuantBlockLanes) * a.scales_hidden_stride] = scale;
-        q[v] = quantize8<kFormat>(y[u], Divisor(scale));
+        store_codes<kNorm>(q + v, quantize8<kFormat>(y[u], Divisor(scale)));
       }
     }
   }
