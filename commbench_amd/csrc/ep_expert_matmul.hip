@@ -8,7 +8,7 @@
 // What bounds it depends on the rows of an expert.  Few rows: reading the weights once (256 experts x 4096 x 7168 with 2 rows
 // each 1071 us, 7.0 TB/s; with 32 rows 1126).  Hundreds: the matrix units at the clock that the card's power limit leaves
 // them (8192^3 442 us, 2490 TOP/s, clock near 1.6 GHz), less what ragged heights leave empty: a segment is computed in
-// blocks of 64 rows (8192 tokens' 65536 rows over 256 experts x 4096 x 7168: 2570 us, of which the empty part of the
+// blocks of 64 rows (8192 tokens' 65536 rows over 256 experts x 4096 x 7168: 2390 us, of which the empty part of the
 // blocks is an eighth).
 #include <atomic>
 #include <type_traits>
@@ -190,23 +190,30 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
 constexpr int kBigN = 256;       // channels of a tile: with kSilu 128 gate channels and their 128 up channels
 constexpr int kBlockRows = 64;   // a tile's rows come in pairs of 32-row blocks, one for each half of the waves
 constexpr int kMaxBlocks = 4;    // 256 rows: the accumulators fill the matrix units' own registers
+// With silu 257 to 320 rows make tall tiles, of all of them and half the channels, so that weights are read once and not by
+// two row tiles that soon drift apart.  Without / with them in us, 128 experts of 264 rows: 4096 x 7168 1676 / 1517, 4096 x
+// 1024 286 / 273; of 384 and 448 rows 4096 x 7168: 1575 / 1748, 1636 / 1943.  Without silu, where a tile has twice the
+// results, they gain with a large inner size only (4096 x 4096 965 / 860, 7168 x 2048 719 / 759), and their being there costs
+// every other shape 1 to 2 %.
+constexpr int kTallBlocks = 5;
 constexpr int kBigThreads = 256;
 constexpr int kRowGroup = 8;
 // A stage of the ring is 128 bytes of k: of the channels (32 KiB), then of the rows (8 KiB for 64 of them).  Tiles of few
 // rows wait for memory and have room for a third stage.
-constexpr int kBBytes = kBigN * kStageK;
 constexpr int kRingBytes = 144 * 1024;
-__host__ __device__ constexpr int stage_bytes_of(int blocks) { return kBBytes + blocks * kBlockRows * kStageK; }
+__host__ __device__ constexpr int channels_of(int blocks) { return blocks <= kMaxBlocks ? kBigN : kBigN / 2; }
+__host__ __device__ constexpr int stage_bytes_of(int blocks) { return (channels_of(blocks) + blocks * kBlockRows) * kStageK; }
 __host__ __device__ constexpr int stages_of(int blocks) { return blocks <= 2 ? 3 : 2; }
-static_assert(stages_of(1) * stage_bytes_of(1) <= kRingBytes && stages_of(2) * stage_bytes_of(2) <= kRingBytes &&
-                  stages_of(3) * stage_bytes_of(3) <= kRingBytes && stages_of(4) * stage_bytes_of(4) <= kRingBytes,
+constexpr bool ring_holds(int blocks) { return stages_of(blocks) * stage_bytes_of(blocks) <= kRingBytes; }
+static_assert(ring_holds(1) && ring_holds(2) && ring_holds(3) && ring_holds(4) && ring_holds(5),
               "the ring");
 // Results of up to this many bytes are written through into the 256 MB memory-side cache where the weights pass that cache
 // by (256 x 64 rows x 4096, 134 MB, k 4096: 698 us, streamed 737); more would push one another out (256 x 128 rows x 7168,
 // 470 MB, k 2048: 840, streamed 768), and so do weights that go through it (8192^3: 471, streamed 442).
 constexpr long long kCachedOutput = 192LL << 20;
 constexpr int kTableAt = kRingBytes;    // row tiles before every thread's experts
-constexpr int kRowScaleBytes = kMaxBlocks * kBlockRows * 4;
+constexpr int kRowScaleBytes = 2 * kBigThreads * 4;
+static_assert(kTallBlocks * kBlockRows * 4 <= kRowScaleBytes, "a tile's row scales");
 constexpr int kScaleBytes = kRowScaleBytes + kBigN * 4;
 constexpr int kScalesAt = kTableAt + (kBigThreads + 4) * 4;  // two tiles' row and channel scales
 constexpr int kBigLds = kScalesAt + 2 * kScaleBytes;
@@ -252,22 +259,31 @@ struct BigMatmul {
         steps((args.in_features + kStageK - 1) / kStageK),
         stream_output(static_cast<long long>(args.num_rows) * columns > kCachedOutput / 2) {}
 
+  // Channels of a tile as 32-wide blocks of a wave, of a matrix, and as output columns.
+  template <int kBlocks>
+  static constexpr int kChannels = channels_of(kBlocks) / 64;
+  template <int kBlocks>
+  static constexpr int kOut = channels_of(kBlocks) / (kSilu ? 2 : 1);
+
   // Load j of stage `step`, whose place in the ring is `slot`: eight rows of the channels, or of the tokens.
-  template <bool kOnce>
+  template <bool kOnce, int kPerWave>
   __device__ __forceinline__ void load_b(const Place& at, int slot, int step, int j) const {
-    const int row = (kSilu ? wave & 1 : wave) * 64 + at.row + j * 8, piece = at.piece_of(j);
-    load_to_lds<kOnce>(desc_b, lds_base + slot + (wave * 8 + j) * kChunkBytes,
+    const int row = (kSilu ? wave & 1 : wave) * (8 * kPerWave) + at.row + j * 8, piece = at.piece_of(j);
+    load_to_lds<kOnce>(desc_b, lds_base + slot + (wave * kPerWave + j) * kChunkBytes,
                        step * kStageK + piece < K ? row * K + piece : kOutside, step * kStageK);
   }
   __device__ __forceinline__ void load_a(const Place& at, int slot, int step, int j) const {
     const int eight = (j >> 1) * 8 + wave * 2 + (j & 1), piece = at.piece_of(j);
-    load_to_lds(desc_a, lds_base + slot + kBBytes + eight * kChunkBytes,
+    load_to_lds(desc_a, lds_base + slot + eight * kChunkBytes,
                 step * kStageK + piece < K ? (eight * 8 + at.row) * K + piece : kOutside, step * kStageK);
   }
 
   // Points the descriptors at a tile and starts the loads of its scales and of its first stages, as many as the ring holds.
   __device__ __forceinline__ void start(const BigTile& tile, int scales_at) {
-    const int b_rows = columns - tile.column < kColumns ? columns - tile.column : kColumns;
+    const int blocks = (tile.rows + kBlockRows - 1) / kBlockRows;
+    const bool tall = kSilu && blocks > kMaxBlocks;
+    const int channels = tall ? kBigN / 2 : kBigN, width = tall ? kColumns / 2 : kColumns, left = columns - tile.column;
+    const int b_rows = left >= width ? width : tall && left < 0 ? 0 : left;
     const size_t channel = static_cast<size_t>(tile.expert) * a.out_features + (kSilu && wave >= 2 ? columns : 0) + tile.column;
     desc_a = descriptor_of(a.a + static_cast<size_t>(tile.first) * K, tile.rows * K);
     desc_b = descriptor_of(a.b + channel * K, b_rows * K);
@@ -277,61 +293,70 @@ struct BigMatmul {
     const int4v desc_scales = descriptor_of(a.a_scales + static_cast<size_t>(tile.first) * a.a_scales_row_stride,
                                             ((tile.rows - 1) * stride + 1) * 4);
     load_word_to_lds(desc_scales, scales_at + wave * 256, row < tile.rows ? row * stride * 4 : kOutside);
+    if constexpr (kSilu)
+      load_word_to_lds(desc_scales, scales_at + (kBigThreads + wave * 64) * 4,
+                       row + kBigThreads < tile.rows ? (row + kBigThreads) * stride * 4 : kOutside);
     load_word_to_lds(descriptor_of(a.b_scales + channel, b_rows * 4), scales_at + kRowScaleBytes + wave * 256,
                      (kSilu ? row & 127 : row) * 4);
-    const int blocks = (tile.rows + kBlockRows - 1) / kBlockRows;
-    const int stages = stages_of(blocks);
+    const int stages = stages_of(blocks), stage_bytes = (channels + blocks * kBlockRows) * kStageK;
     for (int s = 0; s < stages && s < steps; ++s) {
-      const int slot = s * stage_bytes_of(blocks);
-      if (tile.only != 0) {
+      const int slot = s * stage_bytes;
+      if (tall) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) load_b<true>(at, slot, s, j);
+        for (int j = 0; j < 4; ++j) load_b<true, 4>(at, slot, s, j);
+      } else if (tile.only != 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load_b<true, 8>(at, slot, s, j);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) load_b<false>(at, slot, s, j);
+        for (int j = 0; j < 8; ++j) load_b<false, 8>(at, slot, s, j);
       }
 #pragma unroll
-      for (int j = 0; j < 2 * kMaxBlocks; ++j)
-        if (j < 2 * blocks) load_a(at, slot, s, j);
+      for (int j = 0; j < 2 * (kSilu ? kTallBlocks : kMaxBlocks); ++j)
+        if (j < 2 * blocks) load_a(at, slot + channels * kStageK, s, j);
     }
   }
 
   template <int kBlocks>
   struct Fragments {
-    int4v a[2][kBlocks], b[2][4];
+    int4v a[2][kBlocks], b[2][kChannels<kBlocks>];
   };
-  // Fragment i of a quarter of a stage: four of channels, then the rows'.  Lane l takes row l % 32 of a block and
+  // Fragment i of a quarter of a stage: the wave's channels, then the rows.  Lane l takes row l % 32 of a block and
   // piece 2 * quarter + l / 32.
   template <int kBlocks>
   __device__ __forceinline__ void read(const Place& at, Fragments<kBlocks>& f, int slot, int quarter, int i) const {
+    constexpr int kCh = kChannels<kBlocks>;
     const unsigned char* base = lds + slot + (at.read_at ^ (quarter * 32));
-    if (i < 4) {
-      const int block = kSilu ? (i & 1) + nw * 2 + (i >> 1) * 4 : nw * 4 + i;
+    if (i < kCh) {
+      const int block = kSilu ? i % (kCh / 2) + nw * (kCh / 2) + i / (kCh / 2) * kCh : nw * kCh + i;
       f.b[quarter & 1][i] = *reinterpret_cast<const int4v*>(base + block * 32 * kStageK);
     } else {
-      f.a[quarter & 1][i - 4] = *reinterpret_cast<const int4v*>(base + kBBytes + (2 * (i - 4) + mw) * 32 * kStageK);
+      f.a[quarter & 1][i - kCh] =
+          *reinterpret_cast<const int4v*>(base + (channels_of(kBlocks) + (2 * (i - kCh) + mw) * 32) * kStageK);
     }
   }
 
-  enum Loads { kNone, kChannels, kRows };
+  enum Loads { kNone, kWeights, kRows };
   // A quarter of a stage's products; between them, spread over them, the reads of the next quarter's fragments (from
   // the stage in `from`, or with kRead false none) and the loads of a part of stage `ahead` (to `to`).
   template <int kBlocks, bool kOnce, int kQuarter, Loads kLoad, bool kRead = true>
-  __device__ __forceinline__ void quarter(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][4], int from, int to,
+  __device__ __forceinline__ void quarter(const Place& at, Fragments<kBlocks>& f, int16v (&acc)[kBlocks][kChannels<kBlocks>], int from, int to,
                                           int ahead) const {
-    constexpr int kLoads = kLoad == kNone ? 0 : kLoad == kChannels ? 8 : 2 * kBlocks;
-    constexpr int kProducts = 4 * kBlocks, kItems = (kRead ? 4 + kBlocks : 0) + kLoads;
+    constexpr int kCh = kChannels<kBlocks>;
+    constexpr int kLoads = kLoad == kNone ? 0 : kLoad == kWeights ? 2 * kCh : 2 * kBlocks;
+    constexpr int kProducts = kCh * kBlocks, kItems = (kRead ? kCh + kBlocks : 0) + kLoads;
 #pragma unroll
     for (int p = 0; p < kProducts; ++p) {
 #pragma unroll
       for (int i = p * kItems / kProducts; i < (p + 1) * kItems / kProducts; ++i) {
         const int loads_before = kLoads == 0 ? 0 : (i + 1) * kLoads / kItems;
         const bool is_load = kLoads != 0 && loads_before != i * kLoads / kItems;
-        if (is_load) kLoad == kChannels ? load_b<kOnce>(at, to, ahead, loads_before - 1) : load_a(at, to, ahead, loads_before - 1);
+        if (is_load) kLoad == kWeights ? load_b<kOnce, 2 * kCh>(at, to, ahead, loads_before - 1)
+                                   : load_a(at, to + channels_of(kBlocks) * kStageK, ahead, loads_before - 1);
         else read<kBlocks>(at, f, from, (kQuarter + 1) & 3, i - loads_before);
       }
       constexpr int h = kQuarter & 1;
-      acc[p / 4][p % 4] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[h][p % 4], f.a[h][p / 4], acc[p / 4][p % 4], 0, 0, 0);
+      acc[p / kCh][p % kCh] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.b[h][p % kCh], f.a[h][p / kCh], acc[p / kCh][p % kCh], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -341,20 +366,21 @@ struct BigMatmul {
   template <int kBlocks, bool kOnce>
   __device__ __forceinline__ void run(const BigTile& tile, int scales_at, bool has_next, const BigTile& next, int next_scales_at) {
     const Place at(fresh(lane));
-    int16v acc[kBlocks][4];
+    constexpr int kCh = kChannels<kBlocks>;
+    int16v acc[kBlocks][kCh];
     Fragments<kBlocks> f;
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[m][j] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+      for (int j = 0; j < kCh; ++j) acc[m][j] = int16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 
-    constexpr int kStages = stages_of(kBlocks), kStageBytes = stage_bytes_of(kBlocks), kStageLoads = 8 + 2 * kBlocks;
+    constexpr int kStages = stages_of(kBlocks), kStageBytes = stage_bytes_of(kBlocks), kStageLoads = 2 * kCh + 2 * kBlocks;
     if (steps >= kStages)
       wait_and_meet<(kStages - 1) * kStageLoads + kStores>();
     else
       wait_and_meet<kStores>();
 #pragma unroll
-    for (int i = 0; i < 4 + kBlocks; ++i) read<kBlocks>(at, f, 0, 0, i);
+    for (int i = 0; i < kCh + kBlocks; ++i) read<kBlocks>(at, f, 0, 0, i);
     quarter<kBlocks, kOnce, 0, kNone>(at, f, acc, 0, 0, 0);
     quarter<kBlocks, kOnce, 1, kNone>(at, f, acc, 0, 0, 0);
     quarter<kBlocks, kOnce, 2, kNone>(at, f, acc, 0, 0, 0);
@@ -366,7 +392,7 @@ struct BigMatmul {
     const auto go_on = [&](auto load) {
       constexpr bool kLoad = decltype(load)::value;
       const int next_slot = after(here), ahead = step + kStages;
-      quarter<kBlocks, kOnce, 3, kLoad ? kChannels : kNone>(at, f, acc, next_slot, here, ahead);
+      quarter<kBlocks, kOnce, 3, kLoad ? kWeights : kNone>(at, f, acc, next_slot, here, ahead);
       quarter<kBlocks, kOnce, 0, kLoad ? kRows : kNone>(at, f, acc, next_slot, here, ahead);
       quarter<kBlocks, kOnce, 1, kNone>(at, f, acc, next_slot, 0, 0);
       quarter<kBlocks, kOnce, 2, kNone>(at, f, acc, next_slot, 0, 0);
@@ -401,8 +427,8 @@ struct BigMatmul {
 #pragma unroll
     for (int m = 0; m < kBlocks; ++m) row_scale[m] = row_scales[(2 * m + mw) * 32 + r];
 #pragma unroll
-    for (int j = 0; j < (kSilu ? 2 : 4); ++j) {
-      const int column0 = nw * (kSilu ? 64 : 128) + j * 32;  // in the tile
+    for (int j = 0; j < (kSilu ? kCh / 2 : kCh); ++j) {
+      const int column0 = nw * (kOut<kBlocks> / 2) + j * 32;  // in the tile
       float4 s[4], u[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -423,7 +449,7 @@ struct BigMatmul {
             const float ug[4] = {u[g].x, u[g].y, u[g].z, u[g].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + 2) & 3][g * 4 + i]) * (row_scale[m] * ug[i]));
+              o[i] = silu(o[i]) * (static_cast<float>(acc[m][(j + kCh / 2) % kCh][g * 4 + i]) * (row_scale[m] * ug[i]));
           }
           w[g][0] = to_bf16_pair(o[0], o[1]);
           w[g][1] = to_bf16_pair(o[2], o[3]);
@@ -453,7 +479,7 @@ struct BigMatmul {
         __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: more would not fit the registers
       }
     }
-    idle_stores<(kMaxBlocks - kBlocks) * kStores / kMaxBlocks>(out);
+    idle_stores<kStores - 2 * kBlocks * (kSilu ? kCh / 2 : kCh)>(out);
   }
 
   // The waits of the next tile's first steps count the stores of this one, so every tile issues as many: rows
@@ -522,6 +548,8 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
     const Segment all = segment_of(a, expert);
     const int rows = __builtin_amdgcn_readfirstlane(all.rows);
     const int blocks = (rows + kBlockRows - 1) / kBlockRows, row_tiles = row_tiles_of(blocks);
+    if (kSilu && blocks == kTallBlocks)  // in the place of two row tiles
+      return BigTile{expert, (index - first_tile * column_tiles) * (kColumns / 2), __builtin_amdgcn_readfirstlane(all.first), rows, 1};
     // Inside an expert: groups of up to eight row tiles by as many columns as make about 32 tiles, one die's share
     // at a time, so that rows and weights are each fetched once for all of them; columns fastest, so that a
     // group's shorter tiles are shared out over all compute units and not always to the same ones.
@@ -572,7 +600,10 @@ __global__ __launch_bounds__(kBigThreads, 1) void ep_expert_matmul_big_kernel(co
       case 1: matmul.template run<1, true>(tile, at, has_next, next, next_at); break;
       case 2: matmul.template run<2, true>(tile, at, has_next, next, next_at); break;
       case 3: matmul.template run<3, true>(tile, at, has_next, next, next_at); break;
-      default: matmul.template run<4, true>(tile, at, has_next, next, next_at); break;
+      case 4: matmul.template run<4, true>(tile, at, has_next, next, next_at); break;
+      default:
+        if constexpr (kSilu) matmul.template run<5, true>(tile, at, has_next, next, next_at);
+        break;
     }
     else switch (blocks) {  // the shares of at least five blocks
       case 2: matmul.template run<2, false>(tile, at, has_next, next, next_at); break;

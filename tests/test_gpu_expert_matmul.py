@@ -102,6 +102,21 @@ def test_large_tiles_against_integers(n, k, silu):
     assert torch.equal(run_raw(p, silu), out)                         # and the same again, to the bit
 
 
+@pytest.mark.parametrize("k", [112, 128, 272, 640])
+@pytest.mark.parametrize("n,silu", [(520, False), (1296, True), (896, True)])
+def test_tall_tiles_against_integers(n, k, silu):
+    """Segments between one and two tiles' rows, the limits on both sides, next to others."""
+    counts = [448, 449, 0, 320, 319, 384, 447, 256, 258, 20, 440, 383, 450, 511]
+    print(f"tall tiles out {n} in {k} silu {silu}", flush=True)
+    p = problem(n + 3 * k, counts, n, k, extra_rows=9)
+    want, bound, mine = reference(p, silu)
+    p["sa"][~mine] = np.nan
+    out = run_raw(p, silu)
+    xu.check_within(xu.f64(out)[mine], want[mine], bound[mine])
+    assert bool((out.cpu()[torch.from_numpy(~mine)] == -77.0).all())
+    assert torch.equal(run_raw(p, silu), out)
+
+
 @pytest.mark.parametrize("align", [16, 128])
 def test_large_tiles_with_pads_strided_scales_and_without_counts(align):
     p = problem(77, LARGE, 768, 272, align)
