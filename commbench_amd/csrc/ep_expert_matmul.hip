@@ -229,8 +229,8 @@ struct BigTile {
   int only;            // no other tile has rows of the expert
 };
 
-// One workgroup's walk over its tiles.  Wave (mw, nw) owns the 32-row blocks mw, mw + 2, ... and 128 of the 256
-// channels (with kSilu 64 gate channels and the 64 up channels of the same columns).
+// One workgroup's walk over its tiles.  Wave (mw, nw) owns the 32-row blocks mw, mw + 2, ... and half, 128, of the 256
+// channels (with kSilu 64 gate channels and the 64 up channels of the same columns; of a tall tile half as many).
 template <bool kSilu>
 struct BigMatmul {
   static constexpr int kColumns = kSilu ? kBigN / 2 : kBigN;  // output columns of a tile
