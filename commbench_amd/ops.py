@@ -567,7 +567,14 @@ def _check_row_limit(row_limit: Optional[torch.Tensor], device: torch.device) ->
 def _empty_scales(rows: int, groups: int, device: torch.device, column_major: bool) -> torch.Tensor:
     if column_major:
         return torch.empty((groups, rows), dtype=torch.float32, device=device).t()
-    return torch.empty((rows, groups), dtype=torch.float32, device=device)
+    return torch.empty_strided((rows, groups), (groups, 1), dtype=torch.float32, device=device)
+
+
+def _rows_like(x: torch.Tensor, rows: int, row_stride: int, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous matrix of x's shape.  empty_like takes 0.5 us less than empty, but keeps the stride of a single row."""
+    if rows > 1 and row_stride == x.shape[1]:
+        return torch.empty_like(x, dtype=dtype)
+    return torch.empty(x.shape, dtype=dtype, device=x.device)
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -593,13 +600,13 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
         r_rows, r_hidden, r_stride, r_at = _check_rows(residual, "residual")
         _require(r_rows == T and r_hidden == H and residual.device == dev, "residual must have the shape and device of x")
         _require(not update_residual or r_stride == H, "a residual updated in place must be contiguous")
-        out_residual = residual if update_residual else torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+        out_residual = residual if update_residual else _rows_like(x, T, x_stride, torch.bfloat16)
         out_at = out_residual.data_ptr()
     else:
         _require(not update_residual, "update_residual needs a residual")
-    q = torch.empty((T, H), dtype=dtype, device=dev)
+    q = _rows_like(x, T, x_stride, dtype)
     scales = _empty_scales(T, groups, dev, column_major_scales)
-    out_normed = torch.empty((T, H), dtype=torch.bfloat16, device=dev) if normed else None
+    out_normed = _rows_like(x, T, x_stride, torch.bfloat16) if normed else None
     row_stride, hidden_stride = scales.stride()
     _launch(dev, "mi_ep_rms_norm_quantize", x_at, x_stride, r_at, r_stride, g_at,
             struct.unpack("<I", struct.pack("<f", eps))[0], T, H, fmt, q.data_ptr(), scales.data_ptr(), row_stride, hidden_stride,
@@ -618,7 +625,7 @@ def quantize_rows(x: torch.Tensor, quant: str = "int8", row_limit: Optional[torc
     fmt, dtype, groups = _quant_format(quant, H)
     dev = x.device
     limit = _check_row_limit(row_limit, dev)
-    q = torch.empty((rows, H), dtype=dtype, device=dev)
+    q = _rows_like(x, rows, x_stride, dtype)
     scales = _empty_scales(rows, groups, dev, column_major_scales)
     row_stride, hidden_stride = scales.stride()
     _launch(dev, "mi_ep_quantize_rows", x_at, x_stride, limit, rows, H, fmt, q.data_ptr(), scales.data_ptr(), row_stride,
@@ -639,7 +646,7 @@ def dequantize_rows(q: torch.Tensor, scales: torch.Tensor, row_limit: Optional[t
     _require(scales.dtype is torch.float32 and scales.shape == (rows, groups) and scales.device == dev,
              "scales must be a float32 [rows, groups] tensor or view on the device of q")
     limit = _check_row_limit(row_limit, dev)
-    out = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
+    out = _rows_like(q, rows, H, torch.bfloat16)
     row_stride, hidden_stride = scales.stride()
     _launch(dev, "mi_ep_dequantize_rows", q.data_ptr(), scales.data_ptr(), row_stride, hidden_stride, limit, rows, H, fmt,
             out.data_ptr())
