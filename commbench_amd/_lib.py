@@ -51,7 +51,7 @@ SIGNATURES = {
     "mi_ep_dequantize_rows": (_int, [_vp, _vp, ctypes.c_longlong, ctypes.c_longlong, _vp, _int, _int, _int, _vp, _vp]),
     "mi_ep_grouped_matmul_int8": (_int, [_vp, _vp, ctypes.c_longlong, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _vp,
                                          _int, _vp]),
-    "mi_ep_moe_few_tokens_workspace_bytes": (_size, [_int, _int, _int]),
+    "mi_ep_moe_few_tokens_workspace_bytes": (_size, [_int, _int, _int, _int]),
     "mi_ep_moe_few_tokens": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _int, _vp, _vp,
                                     _size, _vp]),
     "mi_ep_host_get_dispatch_layout": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int]),

@@ -695,10 +695,11 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
   return status_of(launch_expert_matmul(m, as_stream(stream)));
 }
 
-size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int intermediate) {
-  if (!few_tokens_shape_ok(num_tokens, num_topk) || intermediate <= 0 || intermediate % 16 != 0 || intermediate > 65536)
+size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int hidden, int intermediate) {
+  if (!few_tokens_shape_ok(num_tokens, num_topk) || intermediate <= 0 || intermediate % 16 != 0 || intermediate > 65536 ||
+      hidden <= 0 || hidden % 16 != 0 || hidden > 65536)
     return 0;
-  return static_cast<size_t>(num_tokens) * num_topk * intermediate * 4;
+  return static_cast<size_t>(num_tokens) * num_topk * (static_cast<size_t>(intermediate) + hidden) * 4;
 }
 
 int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* topk_weights, const void* w13,
@@ -716,7 +717,7 @@ int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* to
   if (num_tokens == 0) return MI_EP_OK;
   if (x == nullptr || topk_idx == nullptr || w13 == nullptr || w2 == nullptr || combined_x == nullptr || workspace == nullptr)
     return MI_EP_EINVAL;
-  if (workspace_bytes < mi_ep_moe_few_tokens_workspace_bytes(num_tokens, num_topk, intermediate)) return MI_EP_ENOSPC;
+  if (workspace_bytes < mi_ep_moe_few_tokens_workspace_bytes(num_tokens, num_topk, hidden, intermediate)) return MI_EP_ENOSPC;
   FewTokensArgs a{};
   a.x = static_cast<const uint16_t*>(x);
   a.topk_idx = topk_idx;
@@ -728,6 +729,7 @@ int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* to
   a.bias_0 = static_cast<const uint16_t*>(bias_0);
   a.bias_1 = static_cast<const uint16_t*>(bias_1);
   a.act = static_cast<uint16_t*>(workspace);
+  a.y = reinterpret_cast<float*>(a.act + static_cast<size_t>(num_tokens) * num_topk * intermediate * 2);
   a.combined_x = static_cast<uint16_t*>(combined_x);
   a.num_tokens = num_tokens;
   a.num_topk = num_topk;

@@ -266,6 +266,7 @@ struct FewTokensArgs {
   const uint16_t* bias_0;
   const uint16_t* bias_1;
   uint16_t* act;  // bf16 [2, num_tokens * num_topk, intermediate]: two terms of every value
+  float* y;       // [num_tokens * num_topk, hidden]: the products of every route, where a sum of its own adds them
   uint16_t* combined_x;
   int num_tokens;
   int num_topk;

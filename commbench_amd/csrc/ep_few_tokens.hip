@@ -1,11 +1,10 @@
-// The whole expert layer for a few tokens in two kernels, for gfx950:
+// The whole expert layer for a few tokens in two or three kernels, for gfx950:
 //   act[r, i] = silu(Wg[e] x[t])[i] * (Wu[e] x[t])[i]                     r = route (t, k) to expert e
 //   out[t, :] = sum_k w[t, k] * W2[e_k] act[(t, k), :] (+ biases)
 // With a few tokens every expert sees one or a handful of rows, so the time is that of reading the met
 // experts' weights once; moving rows to the experts and back would only add launches.  48 tokens of top 8 over 256
-// experts, 7168 x 2048 int8, read 9.0 GB in 1407 us (6.4 TB/s; the first kernel at 6.7, the second at 5.9), 16 tokens
-// over 128 experts, 4096 x 1408 bf16, 2.9 GB in 528 us; one token's 352 MB take 75 us, where starting and draining two
-// kernels shows.  Weights are
+// experts, 7168 x 2048 int8, read 8.7 GB in 1329 us (6.5 TB/s), 16 tokens over 128 experts, 4096 x 1408 bf16, 2.9 GB
+// in 529 us; one token's 352 MB take 75 us, where starting and draining two kernels shows.  Weights are
 // bf16, or int8 with a scale for each output channel (widened to bf16 in registers, exactly), products
 // run on the matrix units with the weights as the 16-row operand and up to 16 of an expert's routes as
 // the columns, sums are fp32.  act is kept as the sum of two bf16 values (16 bits: one alone would be as large an
@@ -353,38 +352,50 @@ __global__ __launch_bounds__(kFirstThreads, 4) void ep_few_tokens_gate_up_kernel
   }
 }
 
-// Gate and up where there are many (entry, 64 columns of act) items: workgroup b takes the b-th contiguous share of them.
-// Wave w owns channels 16 w .. 16 w + 15 of an item's gate and up rows.  A stage is 128 bytes of k of the 128 weight rows
-// and the entry's vectors over the same k; it comes by loads of whole lines past the registers and past the memory-side
-// cache, which is what the memory delivers fastest (half a line at a time, as the products' layout has it for loads into
-// registers, the streaming hint costs: 48 tokens 1850 us with it, 1560 without).  The stages of an item and of the next run on in one ring of three.
-constexpr int kSliceColumns = 64, kTileRing = 3;
-constexpr int kTileVectorsAt = 2 * kSliceColumns * kStageK;            // 16 vectors behind the weights, 1 KiB for four of them
-constexpr int kTileStage = kTileVectorsAt + 4 * kChunkBytes;
-constexpr int kTileScalesAt = kTileRing * kTileStage;                  // two items' scales, 256 bytes a wave
-constexpr int kTileMeetingAt = kTileScalesAt + 2 * kFirstWaves * 256;
-static_assert(kTileScalesAt >= 2 * kMaxExperts * static_cast<int>(sizeof(int)), "scratch of the meeting");
+// Either product where there are many (entry, 128 weight rows) items: workgroup b takes the b-th contiguous share of them.
+// An item's rows are two sets of 64: the gate and the up rows of 64 columns of act, or (kDown) 128 columns of the output; wave
+// w owns rows 16 w .. 16 w + 15 of each.  A stage is 128 bytes of k of the rows and the entry's vectors (kDown: both terms)
+// over the same k; it comes by loads of whole lines past the registers and past the memory-side cache, which is what the
+// memory delivers fastest (half a line at a time, as the products' layout has it for loads into registers, the streaming hint
+// costs: 48 tokens 1850 us with it, 1560 without).  The stages of an item and of the next run on in one ring of three.
+// kDown leaves y = W2[e] act as fp32 for every route; the sum over a token's slots is a kernel of its own.
+constexpr int kSetRows = 64, kTileRing = 3;
+constexpr int kTileVectorsAt = 2 * kSetRows * kStageK;                 // 16 vectors behind the weights, 1 KiB for four of them
+template <bool kDown>
+constexpr int kTileParts = kDown ? 2 : 1;
+template <bool kDown>
+constexpr int kTileStage = kTileVectorsAt + kTileParts<kDown> * 4 * kChunkBytes;
+template <bool kDown>
+constexpr int kTileScalesAt = kTileRing * kTileStage<kDown>;           // two items' scales, 256 bytes a wave
+template <bool kDown>
+constexpr int kTileMeetingAt = kTileScalesAt<kDown> + 2 * kFirstWaves * 256;
+static_assert(kTileScalesAt<false> >= 2 * kMaxExperts * static_cast<int>(sizeof(int)), "scratch of the meeting");
 
-template <bool kInt8>
-__global__ __launch_bounds__(kFirstThreads, 2) void ep_few_tokens_gate_up_tiles_kernel(const FewTokensArgs a) {
+template <bool kInt8, bool kDown>
+__global__ __launch_bounds__(kFirstThreads, 2) void ep_few_tokens_tiles_kernel(const FewTokensArgs a) {
   constexpr int kBytes = kInt8 ? 1 : 2;
   constexpr int kElements = kStageK / kBytes;      // of k in a stage
   constexpr int kVectorBytes = 2 * kElements;      // of a column in a stage
   constexpr int kPieces = kVectorBytes / 16;       // 16 (int8 weights) or 8
-  constexpr int kLoads = 5, kStores = 2;           // of a wave: for a stage, for an item's results
+  constexpr int kParts = kTileParts<kDown>, kStage = kTileStage<kDown>, kScalesAt = kTileScalesAt<kDown>;
+  constexpr int kLoads = 4 + kParts, kStores = 2;  // of a wave: for a stage, for an item's results
+  constexpr int kItemColumns = kDown ? 2 * kSetRows : kSetRows;
   extern __shared__ __align__(1024) unsigned char lds[];
   __shared__ uint16_t lists[kFirstWaves][16];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int routes = a.num_tokens * a.num_topk;
   Meeting<16> meeting;
-  meeting.make(a, routes, lds + kTileMeetingAt, reinterpret_cast<int*>(lds));
+  meeting.make(a, routes, lds + kTileMeetingAt<kDown>, reinterpret_cast<int*>(lds));
 
-  const int H = a.hidden, I = a.intermediate;
-  const int slices = (I + kSliceColumns - 1) / kSliceColumns;
+  const int inner = kDown ? a.intermediate : a.hidden;
+  const int columns = kDown ? a.hidden : a.intermediate;          // of the result
+  const int weight_rows = kDown ? a.hidden : 2 * a.intermediate;  // of an expert
+  const int set_distance = kDown ? kSetRows : a.intermediate;     // rows between the two sets
+  const int slices = (columns + kItemColumns - 1) / kItemColumns;
   const long long items = static_cast<long long>(meeting.count) * slices, workgroups = static_cast<long long>(gridDim.x);
   const int from = static_cast<int>(items * blockIdx.x / workgroups), to = static_cast<int>(items * (blockIdx.x + 1) / workgroups);
   if (from >= to) return;
-  const int steps = (H + kElements - 1) / kElements;
+  const int steps = (inner + kElements - 1) / kElements;
   const Place at(lane);
   const int lds_base = lds_address(lds);
 
@@ -396,58 +407,65 @@ __global__ __launch_bounds__(kFirstThreads, 2) void ep_few_tokens_gate_up_tiles_
   const int read_column = lane & 15;
   const int read_vector = kTileVectorsAt + (read_column >> 2) * kChunkBytes + (read_column & 3) * kVectorBytes;
   const int column[2] = {read_column, load_column};
-  const int4v desc_x = descriptor_of(a.x, a.num_tokens * H * 2);
+  const int4v desc_vectors = kDown ? descriptor_of(a.act, routes * inner * 4) : descriptor_of(a.x, a.num_tokens * inner * 2);
 
   int ahead = from, ahead_step = 0, ahead_entry = -1, ahead_slot = 0;  // where the loads stand
   int next_route[2] = {-1, -1}, route = -1, next_item_route = -1, vector_at = kOutside;
-  int4v desc_gate = desc_x, desc_up = desc_x;
+  int4v desc[2] = {desc_vectors, desc_vectors};
   const auto load_stage = [&]() {
     if (ahead_step == 0 && ahead < to) {
-      const int entry = ahead / slices, e = meeting.expert(entry), i0 = (ahead - entry * slices) * kSliceColumns;
+      const int entry = ahead / slices, e = meeting.expert(entry), first = (ahead - entry * slices) * kItemColumns;
       if (entry != ahead_entry) {
         meeting.template columns<2>(entry, routes, lists[wave], column, next_route);
-        vector_at = next_route[1] >= 0 && load_lane == lane ? next_route[1] / a.num_topk * H * 2 : kOutside;
+        const int vector = kDown ? next_route[1] : next_route[1] / a.num_topk;
+        vector_at = next_route[1] >= 0 && load_lane == lane ? vector * inner * 2 : kOutside;
         ahead_entry = entry;
       }
       next_item_route = next_route[0];
-      const int rows = I - i0 < kSliceColumns ? I - i0 : kSliceColumns;
-      const unsigned char* gate = a.w13 + (static_cast<size_t>(e) * 2 * I + i0) * H * kBytes;
-      desc_gate = descriptor_of(gate, rows * H * kBytes);
-      desc_up = descriptor_of(gate + static_cast<size_t>(I) * H * kBytes, rows * H * kBytes);
-      if constexpr (kInt8) {  // lanes 0 to 15: the wave's gate scales, 16 to 31: its up scales
-        const float* scales = a.w13_scales + static_cast<size_t>(e) * 2 * I;
-        const int row = i0 + wave * 16 + (lane & 15);
-        load_word_to_lds(descriptor_of(scales, 2 * I * 4), lds_base + kTileScalesAt + ((ahead & 1) * kFirstWaves + wave) * 256,
-                         lane < 32 && row < I ? (row + (lane >> 4) * I) * 4 : kOutside);
+      const unsigned char* rows = (kDown ? a.w2 : a.w13) + (static_cast<size_t>(e) * weight_rows + first) * inner * kBytes;
+#pragma unroll
+      for (int set = 0; set < 2; ++set) {
+        const int left = columns - first - (kDown ? set * kSetRows : 0);
+        desc[set] = descriptor_of(rows + static_cast<size_t>(set * set_distance) * inner * kBytes,
+                                  (left < 0 ? 0 : left < kSetRows ? left : kSetRows) * inner * kBytes);
+      }
+      if constexpr (kInt8) {  // lanes 0 to 15: the scales of the wave's rows of the first set, 16 to 31: of the second
+        const float* scales = (kDown ? a.w2_scales : a.w13_scales) + static_cast<size_t>(e) * weight_rows;
+        const int row = first + wave * 16 + (lane & 15), set = lane >> 4;
+        load_word_to_lds(descriptor_of(scales, weight_rows * 4), lds_base + kScalesAt + ((ahead & 1) * kFirstWaves + wave) * 256,
+                         set < 2 && row + (kDown ? set * kSetRows : 0) < columns ? (row + set * set_distance) * 4 : kOutside);
       }
     }
     const int k0 = ahead_step * kStageK;
-    const int to_slot = lds_base + ahead_slot * kTileStage;
+    const int to_slot = lds_base + ahead_slot * kStage;
     const bool live = ahead < to;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int piece = at.piece_of(j);
-      const int offset = live && k0 + piece < H * kBytes ? (wave * 16 + j * 8 + at.row) * H * kBytes + piece : kOutside;
-      load_to_lds<true>(desc_gate, to_slot + (wave * 2 + j) * kChunkBytes, offset, k0);
-      load_to_lds<true>(desc_up, to_slot + (8 + wave * 2 + j) * kChunkBytes, offset, k0);
+      const int offset = live && k0 + piece < inner * kBytes ? (wave * 16 + j * 8 + at.row) * inner * kBytes + piece : kOutside;
+#pragma unroll
+      for (int set = 0; set < 2; ++set)
+        load_to_lds<true>(desc[set], to_slot + (set * 8 + wave * 2 + j) * kChunkBytes, offset, k0);
     }
     const int k = ahead_step * kVectorBytes;
-    load_to_lds(desc_x, to_slot + kTileVectorsAt + wave * kChunkBytes,
-                live && vector_at >= 0 && k + load_piece * 16 < H * 2 ? vector_at + load_piece * 16 : kOutside, k);
+    const int offset = live && vector_at >= 0 && k + load_piece * 16 < inner * 2 ? vector_at + load_piece * 16 : kOutside;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+      load_to_lds(desc_vectors, to_slot + kTileVectorsAt + (part * 4 + wave) * kChunkBytes, offset, k + part * routes * inner * 2);
     ahead_slot = ahead_slot + 1 == kTileRing ? 0 : ahead_slot + 1;
     if (++ahead_step == steps) {
       ahead_step = 0;
       ++ahead;
     }
   };
-  const __amdgpu_buffer_rsrc_t act = rows_of(a.act, routes * I * 4);
+  const __amdgpu_buffer_rsrc_t result = kDown ? rows_of(a.y, routes * columns * 4) : rows_of(a.act, routes * columns * 4);
 
 #pragma unroll
   for (int s = 0; s < kTileRing - 1; ++s) load_stage();
   int slot = 0, since = kTileRing;  // stages since the last results were stored
   for (int item = from; item < to; ++item) {
     // At the start of an item the loads are two stages ahead, still in this item: it has two stages at least.
-    float4v gate = {0, 0, 0, 0}, up = {0, 0, 0, 0};
+    float4v sum[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     for (int step = 0; step < steps; ++step) {
       // This stage is in (the next one and an item's stores may be on their way), and every wave has left the stage before
       // it, whose place the next load takes.
@@ -458,53 +476,90 @@ __global__ __launch_bounds__(kFirstThreads, 2) void ep_few_tokens_gate_up_tiles_
       ++since;
       if (step == 0) route = next_item_route;
       load_stage();
-      const unsigned char* stage = lds + slot * kTileStage;
+      const unsigned char* stage = lds + slot * kStage;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // Rows are permuted by half their number, as Place says.
-        const int piece = ((h * 4 + (lane >> 4)) ^ ((read_column >> 1) & 7)) * 16;
-        const vec16 g = *reinterpret_cast<const vec16*>(stage + (wave * 16 + read_column) * kStageK + piece);
-        const vec16 u = *reinterpret_cast<const vec16*>(stage + (kSliceColumns + wave * 16 + read_column) * kStageK + piece);
-        if constexpr (kInt8) {
+        const int group = h * 4 + (lane >> 4), piece = (group ^ ((read_column >> 1) & 7)) * 16;
+        vec16 w[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int of = (((h * 4 + (lane >> 4)) * 2 + i) ^ read_column) * 16;
-            const bf16x8 x = as_bf16(*reinterpret_cast<const vec16*>(stage + read_vector + of));
-            gate = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(g[2 * i], g[2 * i + 1]), x, gate, 0, 0, 0);
-            up = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(u[2 * i], u[2 * i + 1]), x, up, 0, 0, 0);
+        for (int set = 0; set < 2; ++set)
+          w[set] = *reinterpret_cast<const vec16*>(stage + (set * kSetRows + wave * 16 + read_column) * kStageK + piece);
+#pragma unroll
+        for (int i = 0; i < (kInt8 ? 2 : 1); ++i) {
+          const int of = kInt8 ? ((group * 2 + i) ^ read_column) * 16 : (group ^ (read_column >> 1)) * 16;
+          bf16x8 rows[2];
+#pragma unroll
+          for (int set = 0; set < 2; ++set) rows[set] = kInt8 ? widen(w[set][2 * i], w[set][2 * i + 1]) : as_bf16(w[set]);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            const bf16x8 x = as_bf16(*reinterpret_cast<const vec16*>(stage + read_vector + part * 4 * kChunkBytes + of));
+#pragma unroll
+            for (int set = 0; set < 2; ++set) sum[set] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(rows[set], x, sum[set], 0, 0, 0);
           }
-        } else {
-          const int of = ((h * 4 + (lane >> 4)) ^ (read_column >> 1)) * 16;
-          const bf16x8 x = as_bf16(*reinterpret_cast<const vec16*>(stage + read_vector + of));
-          gate = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(g), x, gate, 0, 0, 0);
-          up = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(u), x, up, 0, 0, 0);
         }
       }
       slot = slot + 1 == kTileRing ? 0 : slot + 1;
     }
-    // Lane l holds channels 4 (l / 16) + 0..3 of column l % 16.
-    const int first = item % slices * kSliceColumns + wave * 16 + (lane >> 4) * 4;
+    // Lane l holds rows 4 (l / 16) + 0..3 of column l % 16.
+    const int first = item % slices * kItemColumns + wave * 16 + (lane >> 4) * 4;
     if constexpr (kInt8) {
-      const float* scales = reinterpret_cast<const float*>(lds + kTileScalesAt + ((item & 1) * kFirstWaves + wave) * 256);
-      const float4 of_gate = *reinterpret_cast<const float4*>(scales + (lane >> 4) * 4);
-      const float4 of_up = *reinterpret_cast<const float4*>(scales + 16 + (lane >> 4) * 4);
-      gate[0] *= of_gate.x, gate[1] *= of_gate.y, gate[2] *= of_gate.z, gate[3] *= of_gate.w;
-      up[0] *= of_up.x, up[1] *= of_up.y, up[2] *= of_up.z, up[3] *= of_up.w;
-    }
-    uint32_t high[4], low[4];
+      const float* scales = reinterpret_cast<const float*>(lds + kScalesAt + ((item & 1) * kFirstWaves + wave) * 256);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) activate(gate[i], up[i], high[i], low[i]);
-    const int offset = route >= 0 && first < I ? (route * I + first) * 2 : kOutside;
-    __builtin_amdgcn_raw_buffer_store_b64(words2{high[0] | high[1] << 16, high[2] | high[3] << 16}, act, offset, 0,
-                                          kCachePolicyDeviceScope);
-    __builtin_amdgcn_raw_buffer_store_b64(words2{low[0] | low[1] << 16, low[2] | low[3] << 16}, act, offset,
-                                          routes * I * 2, kCachePolicyDeviceScope);
+      for (int set = 0; set < 2; ++set) {
+        const float4 of = *reinterpret_cast<const float4*>(scales + set * 16 + (lane >> 4) * 4);
+        sum[set][0] *= of.x, sum[set][1] *= of.y, sum[set][2] *= of.z, sum[set][3] *= of.w;
+      }
+    }
+    if constexpr (kDown) {
+#pragma unroll
+      for (int set = 0; set < 2; ++set) {
+        const int c = first + set * kSetRows;
+        const vec16 bits = {__float_as_uint(sum[set][0]), __float_as_uint(sum[set][1]), __float_as_uint(sum[set][2]),
+                            __float_as_uint(sum[set][3])};
+        __builtin_amdgcn_raw_buffer_store_b128(bits, result, route >= 0 && c < columns ? (route * columns + c) * 4 : kOutside, 0,
+                                               kCachePolicyDeviceScope);
+      }
+    } else {
+      uint32_t high[4], low[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) activate(sum[0][i], sum[1][i], high[i], low[i]);
+      const int offset = route >= 0 && first < columns ? (route * columns + first) * 2 : kOutside;
+      __builtin_amdgcn_raw_buffer_store_b64(words2{high[0] | high[1] << 16, high[2] | high[3] << 16}, result, offset, 0,
+                                            kCachePolicyDeviceScope);
+      __builtin_amdgcn_raw_buffer_store_b64(words2{low[0] | low[1] << 16, low[2] | low[3] << 16}, result, offset,
+                                            routes * columns * 2, kCachePolicyDeviceScope);
+    }
     since = 0;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load outlives the workgroup's LDS
 }
 
-// Down.  Workgroup h: 16 columns of the output for every token.  Items are the entries (with fewer of them than
+// out[t] = sum_k w[t, k] y[(t, k)] + biases, the slots in ascending order; a thread four columns.
+__global__ __launch_bounds__(kFirstThreads) void ep_few_tokens_sum_kernel(const FewTokensArgs a) {
+  const int quads = a.hidden / 4;
+  const int index = static_cast<int>(blockIdx.x) * kFirstThreads + static_cast<int>(threadIdx.x);
+  const int t = index / quads, c = (index - t * quads) * 4;
+  if (t >= a.num_tokens) return;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int k = 0; k < a.num_topk; ++k) {
+    const int r = t * a.num_topk + k;
+    const int64_t e = a.topk_idx[r];
+    if (e < 0 || e >= a.num_experts) continue;
+    const float w = a.topk_weights != nullptr ? a.topk_weights[r] : 1.0f;
+    const float4 v = *reinterpret_cast<const float4*>(a.y + static_cast<size_t>(r) * a.hidden + c);
+    sum[0] = __builtin_fmaf(w, v.x, sum[0]), sum[1] = __builtin_fmaf(w, v.y, sum[1]);
+    sum[2] = __builtin_fmaf(w, v.z, sum[2]), sum[3] = __builtin_fmaf(w, v.w, sum[3]);
+  }
+  const size_t o = static_cast<size_t>(t) * a.hidden + c;
+  for (const uint16_t* bias : {a.bias_0, a.bias_1})
+    if (bias != nullptr)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += bf16_lo(bias[o + i]);
+  *reinterpret_cast<uint2*>(a.combined_x + o) = uint2{to_bf16_pair(sum[0], sum[1]), to_bf16_pair(sum[2], sum[3])};
+}
+
+// Down where there are few items, or many routes for an expert.  Workgroup h: 16 columns of the output for every token.  Items are the entries (with fewer of them than
 // waves, shares of their k); wave w takes items w, w + 8, ...  y[split][route][16] collects the products.
 template <bool kInt8, int kBlocks, int kDepth, int kFold>
 __global__ __launch_bounds__(kSecondThreads, 4) void ep_few_tokens_down_kernel(const FewTokensArgs a, const int splits) {
@@ -625,9 +680,9 @@ hipError_t launch_gate_up(const FewTokensArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <bool kInt8>
-hipError_t launch_gate_up_tiles(const FewTokensArgs& a, int compute_units, hipStream_t stream) {
-  const int lds = kTileMeetingAt + static_cast<int>(Meeting<16>::bytes(a.num_tokens * a.num_topk));
+template <bool kInt8, bool kDown>
+hipError_t launch_tiles(const FewTokensArgs& a, int compute_units, hipStream_t stream) {
+  const int lds = kTileMeetingAt<kDown> + static_cast<int>(Meeting<16>::bytes(a.num_tokens * a.num_topk));
   int ordinal = 0;
   hipError_t e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
   if (e != hipSuccess) return e;
@@ -636,12 +691,12 @@ hipError_t launch_gate_up_tiles(const FewTokensArgs& a, int compute_units, hipSt
   static std::atomic<int> lds_limit_raised[kMaxDevices];
   if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
   if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_gate_up_tiles_kernel<kInt8>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_tiles_kernel<kInt8, kDown>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
     if (e != hipSuccess) return e;
     lds_limit_raised[ordinal].store(1, std::memory_order_release);
   }
-  hipLaunchKernelGGL((ep_few_tokens_gate_up_tiles_kernel<kInt8>), dim3(static_cast<unsigned>(2 * compute_units)),
+  hipLaunchKernelGGL((ep_few_tokens_tiles_kernel<kInt8, kDown>), dim3(static_cast<unsigned>(2 * compute_units)),
                      dim3(kFirstThreads), lds, stream, a);
   return hipGetLastError();
 }
@@ -685,11 +740,24 @@ hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
   // of top 8 over 256 experts, 7168 x 2048 int8 1564 / 1412; 16 over 128, 4096 x 1408 bf16 580 / 531; 4 tokens of the first
   // (1024 items) 271 / 243, one token (256) 76 / 81; 12 tokens of top 4 over 64 experts, 4096 x 1024 (768) 116 / 128.
   const long long met = routes < a.num_experts ? routes : a.num_experts;
-  const long long items = met * ((a.intermediate + kSliceColumns - 1) / kSliceColumns);
-  const bool tiles = !many && a.hidden > kStageK && items >= 4LL * dev.compute_units;
+  const auto tiles = [&](int inner, int columns, int item_columns, int items_for_unit) {
+    const long long items = met * ((columns + item_columns - 1) / item_columns);
+    return !many && inner > kStageK && items >= static_cast<long long>(items_for_unit) * dev.compute_units;
+  };
   e = many ? launch_gate_up<kInt8, 4, 1>(a, stream)
-      : tiles ? launch_gate_up_tiles<kInt8>(a, dev.compute_units, stream) : launch_gate_up<kInt8, 1, 2>(a, stream);
+      : tiles(a.hidden, a.intermediate, kSetRows, 4) ? launch_tiles<kInt8, false>(a, dev.compute_units, stream)
+                                                  : launch_gate_up<kInt8, 1, 2>(a, stream);
   if (e != hipSuccess) return e;
+  // The second product's tiles cost a launch and the traffic of y: 48 tokens (14336 items) 1407 / 1329, 16 tokens (4096) 529 /
+  // 531, 12 tokens (1536) 115 / 122.
+  if (tiles(a.intermediate, a.hidden, 2 * kSetRows, 16)) {
+    e = launch_tiles<kInt8, true>(a, dev.compute_units, stream);
+    if (e != hipSuccess) return e;
+    const long long threads = static_cast<long long>(a.num_tokens) * (a.hidden / 4);
+    hipLaunchKernelGGL(ep_few_tokens_sum_kernel, dim3(static_cast<unsigned>((threads + kFirstThreads - 1) / kFirstThreads)),
+                       dim3(kFirstThreads), 0, stream, a);
+    return hipGetLastError();
+  }
   if (many) return launch_down<kInt8, 4, 1, 1>(a, stream);
   if (routes > 2 * a.num_experts) return launch_down<kInt8, 1, 4, 1>(a, stream);
   return launch_down<kInt8, 1, 4, 2>(a, stream);

@@ -705,7 +705,7 @@ def grouped_matmul_int8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor
 def moe_few_tokens(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: Optional[torch.Tensor], w13: torch.Tensor,
                    w2: torch.Tensor, w13_scales: Optional[torch.Tensor] = None, w2_scales: Optional[torch.Tensor] = None,
                    bias: Union[None, torch.Tensor, Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]] = None):
-    """The whole expert layer for a few tokens (num_tokens * num_topk <= 1024) in two launches:
+    """The whole expert layer for a few tokens (num_tokens * num_topk <= 1024) in two or three launches:
     out[t] = sum_k w[t,k] * W2[e] (silu(Wgate[e] x[t]) * (Wup[e] x[t])) (+ biases), e = topk_idx[t,k].
 
     x is bf16 [tokens, hidden]; w13 [experts, 2 * intermediate, hidden] holds the gate rows, then the up
@@ -747,7 +747,7 @@ def moe_few_tokens(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: Option
                  "bias must be contiguous bf16 [num_tokens, hidden]")
     out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
     # A workspace of the call's own: calls on other streams, and captured graphs, never share one.
-    nbytes = _lib.load().mi_ep_moe_few_tokens_workspace_bytes(T, K, I)
+    nbytes = _lib.load().mi_ep_moe_few_tokens_workspace_bytes(T, K, H, I)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch(dev, "mi_ep_moe_few_tokens", x.data_ptr(), topk_idx.data_ptr(), _ptr(topk_weights), w13.data_ptr(),
             _ptr(w13_scales), w2.data_ptr(), _ptr(w2_scales), _ptr(bias_0), _ptr(bias_1), T, K, E, H, I, out.data_ptr(),

@@ -450,7 +450,7 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
                               int in_features, void* out, int flags, void* stream);
 
 /*
- * The whole expert layer for a few tokens, in two launches and without moving a row:
+ * The whole expert layer for a few tokens, in two or three launches and without moving a row:
  *   combined_x[t] = bf16( sum_k w[t,k] * W2[e] (silu(Wgate[e] x[t]) * (Wup[e] x[t])) + bias_0[t] + bias_1[t] ),
  *   e = topk_idx[t, k]; slots outside [0, num_experts) are no routes, a token without routes gets its biases
  * (zeros without).  It reads the weights of the experts that the tokens met, once; with many tokens dispatch, the
@@ -467,7 +467,7 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
  * at most 65536; x, w13, w2, biases and combined_x 16-byte aligned.
  */
 #define MI_EP_FEW_MAX_ROUTES 1024
-size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int intermediate);
+size_t mi_ep_moe_few_tokens_workspace_bytes(int num_tokens, int num_topk, int hidden, int intermediate);
 int mi_ep_moe_few_tokens(const void* x, const int64_t* topk_idx, const float* topk_weights, const void* w13,
                          const float* w13_scales, const void* w2, const float* w2_scales, const void* bias_0,
                          const void* bias_1, int num_tokens, int num_topk, int num_experts, int hidden,

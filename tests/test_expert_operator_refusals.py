@@ -69,10 +69,11 @@ def test_few_tokens_refuses():
                 dict(h=65552), dict(i=65552), dict(x=A + 2), dict(w13=A + 8), dict(w2=A + 8), dict(b0=A + 2), dict(b1=A + 2), dict(out=A + 8),
                 dict(ws=A + 8)):
         assert few(**bad) == EINVAL, bad
-    assert few(nbytes=4 * 2 * 32 * 4 - 1) == ENOSPC
-    assert lib().mi_ep_moe_few_tokens_workspace_bytes(4, 2, 32) == 4 * 2 * 32 * 4
-    assert lib().mi_ep_moe_few_tokens_workspace_bytes(129, 8, 32) == 0
-    assert lib().mi_ep_moe_few_tokens_workspace_bytes(4, 2, 30) == 0
+    assert few(nbytes=4 * 2 * (32 + 64) * 4 - 1) == ENOSPC
+    assert lib().mi_ep_moe_few_tokens_workspace_bytes(4, 2, 64, 32) == 4 * 2 * (32 + 64) * 4
+    assert lib().mi_ep_moe_few_tokens_workspace_bytes(129, 8, 64, 32) == 0
+    assert lib().mi_ep_moe_few_tokens_workspace_bytes(4, 2, 64, 30) == 0
+    assert lib().mi_ep_moe_few_tokens_workspace_bytes(4, 2, 60, 32) == 0
 
 
 def test_python_surface_refuses_host_tensors_and_wrong_types():

@@ -65,23 +65,32 @@ FOLDS = [  # few routes for each expert, several for one of them; many for one, 
     (40, 64, 4, 160, 64, 0.0, "zipf"), (40, 64, 4, 528, 144, 0.2, "zipf"), (128, 1024, 8, 32, 16, 0.0, "uniform")]
 
 
-TILES = [  # enough experts and columns for the tiles of the first product: two stages and more, ragged columns, several passes
+TILES = [  # enough experts and columns for the tiles of the first product: two stages and more, ragged columns, several
+    # passes, biases, a token without a route
     (128, 1024, 8, 144, 48, 0.0, "uniform"), (128, 1024, 8, 272, 64, 0.1, "zipf"), (64, 512, 4, 400, 272, 0.0, "uniform"),
-    (40, 512, 8, 256, 208, 0.3, "uniform"), (128, 300, 8, 160, 224, 0.05, "zipf"), (16, 256, 8, 1040, 528, 0.0, "uniform")]
+    (40, 512, 8, 256, 208, 0.3, "uniform"), (128, 300, 8, 160, 224, 0.05, "zipf"), (16, 256, 8, 1040, 528, 0.0, "uniform"),
+    (33, 1000, 8, 656, 256, 0.3, "uniform"),
+    (128, 1024, 8, 528, 144, 0.0, "uniform"), (127, 1024, 8, 560, 272, 0.1, "zipf")]   # and for those of the second
 
 
 @pytest.mark.parametrize("T,E,K,H,I,mask,kind", TILES)
 @pytest.mark.parametrize("quantised", [True, False])
-def test_many_items_of_the_first_product(T, E, K, H, I, mask, kind, quantised):
+def test_many_items_of_a_product(T, E, K, H, I, mask, kind, quantised):
     print(f"tokens {T} experts {E} slots {K} hidden {H} intermediate {I} masked {mask} {kind} int8 {quantised}", flush=True)
     assert min(T * K, E) * ((I + 63) // 64) >= 4 * 256
     p = problem(T * 7 + H, T, E, K, H, I, quantised, mask, kind)
-    want, bound = reference(p)
+    rng = np.random.default_rng(T)
+    biases = [xu.bf16_round(rng.standard_normal((T, H))) for _ in range(2)] if T % 2 else []
+    p["ids"][T // 2] = -1                                # a token without a route
+    want, bound = reference(p, True, biases)
     g = on_gpu(p)
-    out = call(g)
+    arg = tuple(b.to(xu.DEV) for b in biases) or None
+    out = call(g, True, arg)
     xu.check_within(xu.f64(out), want, bound)
     for _ in range(3):
-        assert torch.equal(call(g), out)
+        assert torch.equal(call(g, True, arg), out)
+    plain, plain_bound = reference(p, False)
+    xu.check_within(xu.f64(call(g, False)), plain, plain_bound)
 
 
 @pytest.mark.parametrize("T,E,K,H,I,mask,kind", FOLDS)
@@ -219,10 +228,10 @@ def test_captured_graphs_replay_with_new_inputs_next_to_each_other():
 
 def test_workspace_size_is_checked_and_no_tokens_is_no_work():
     lib = _lib.load()
-    assert lib.mi_ep_moe_few_tokens_workspace_bytes(128, 8, 2048) == 128 * 8 * 2048 * 4
+    assert lib.mi_ep_moe_few_tokens_workspace_bytes(128, 8, 7168, 2048) == 128 * 8 * (7168 + 2048) * 4
     g = on_gpu(problem(25, 2, 4, 2, 64, 32, False))
     out = torch.full((2, 64), 5.0, dtype=torch.bfloat16, device=xu.DEV)
-    work = torch.empty(2 * 2 * 32 * 4, dtype=torch.uint8, device=xu.DEV)
+    work = torch.empty(2 * 2 * (32 + 64) * 4, dtype=torch.uint8, device=xu.DEV)
     args = lambda nbytes: (g["x"].data_ptr(), g["ids"].data_ptr(), g["gates"].data_ptr(), g["w13"].data_ptr(), None,
                            g["w2"].data_ptr(), None, None, None, 2, 2, 4, 64, 32, out.data_ptr(), work.data_ptr(), nbytes,
                            torch.cuda.current_stream().cuda_stream)
