@@ -7,7 +7,8 @@
 //
 // A row is read once and stays in registers: one workgroup (rows up to 4096 columns: one wave) owns a
 // row, so the mean and the maximum are two reductions over data that never leave the compute unit.  The
-// sum of squares, the mean and y are fp32; nothing is rounded to bf16 on the way to q.  Bound by HBM: 7
+// sum of squares, the mean and y are fp32; nothing is rounded to bf16 on the way to q.  A row whose sum of squares leaves
+// fp32 at either end is brought near one by a power of two, from the registers, and summed again.  Bound by HBM: 7
 // bytes an element move (x, residual in, residual out, q) for about 25 vector instructions per 8 elements
 // and reduction step.
 #include "ep_device.h"
@@ -46,6 +47,33 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {
   v = umax(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x124, 0xf, 0xf, true)));
   v = umax(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x122, 0xf, 0xf, true)));
   v = umax(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x121, 0xf, 0xf, true)));
+  return v;
+}
+
+// The same over a row's waves, through one word of LDS each.  A second call on the same words needs a barrier between
+// the first's reads and its own writes.
+template <int kWaves>
+__device__ __forceinline__ float row_sum(float v, float* words, int wave) {
+  v = wave_sum(v);
+  if constexpr (kWaves > 1) {
+    if (lane_id() == 0) words[wave] = v;
+    __syncthreads();
+    v = words[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += words[w];
+  }
+  return v;
+}
+template <int kWaves>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* words, int wave) {
+  v = wave_max(v);
+  if constexpr (kWaves > 1) {
+    if (lane_id() == 0) words[wave] = v;
+    __syncthreads();
+    v = words[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v = umax(v, words[w]);
+  }
   return v;
 }
 
@@ -177,15 +205,39 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
     }
   }
   if constexpr (kNorm) {
-    sum = wave_sum(sum);
-    if constexpr (kWaves > 1) {
-      if (lane_id() == 0) sums[wave] = sum;
-      __syncthreads();
-      sum = sums[0];
+    sum = row_sum<kWaves>(sum, sums, wave);
+    float mean = sum / static_cast<float>(a.row_vecs * 8) + a.eps;
+    // Below, squares under the least fp32 value, 2^-149, would count for something (each loses up to 2^-150); above, the
+    // sum has overflowed.  Then the row is divided by a power of two first.  The same for every thread of the row.
+    if (__builtin_expect(!(mean >= 0x1p-120f && mean <= 0x1.fffffep127f), 0)) {
+      uint32_t largest = 0;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) sum += sums[w];
+      for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = umax(largest, __float_as_uint(y[u][i]) & 0x7fffffffu);
+      largest = row_max<kWaves>(largest, maxima, wave);
+      // A row that holds an infinity or a NaN, or nothing but zeros, is left as it is.
+      if (largest != 0 && largest < 0x7f800000u) {
+        // Of the row's largest magnitude and of epsilon's root, whichever is larger is brought near one.
+        int exponent = __builtin_amdgcn_frexp_expf(__uint_as_float(largest));
+        if (a.eps > 0.0f) {
+          const int root = __builtin_amdgcn_frexp_expf(a.eps) >> 1;
+          exponent = exponent > root ? exponent : root;
+        }
+        sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            y[u][i] = __builtin_amdgcn_ldexpf(y[u][i], -exponent);
+            sum = __builtin_fmaf(y[u][i], y[u][i], sum);
+          }
+        sum = row_sum<kWaves>(sum, sums, wave);
+        mean = sum / static_cast<float>(a.row_vecs * 8) + __builtin_amdgcn_ldexpf(a.eps, -2 * exponent);
+      }
+      if constexpr (kWaves > 1) __syncthreads();  // `maxima` and `sums` have been read
     }
-    const float inv = 1.0f / sqrtf(sum / static_cast<float>(a.row_vecs * 8) + a.eps);
+    const float inv = 1.0f / sqrtf(mean);
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       const int v = t + u * kRowThreads;
@@ -212,14 +264,7 @@ __global__ __launch_bounds__(kRowThreads == kWave ? 4 * kWave : kRowThreads) voi
     uint32_t m = amax[0];
 #pragma unroll
     for (int u = 1; u < kVecs; ++u) m = umax(m, amax[u]);
-    m = wave_max(m);
-    if constexpr (kWaves > 1) {
-      if (lane_id() == 0) maxima[wave] = m;
-      __syncthreads();
-      m = maxima[0];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) m = umax(m, maxima[w]);
-    }
+    m = row_max<kWaves>(m, maxima, wave);
     // One value for the whole row: in a scalar register the range test costs no vector instruction.
     const float scale = wave_read(scale_of<kFormat>(m), 0);
     if (t == 0) *scales = scale;

@@ -404,8 +404,9 @@ int mi_ep_combine(const void* y, int num_rows, const int* slot_map, const float*
  *   residual_out bf16 [num_rows, hidden] or NULL: h rounded once.  It may be residual or x themselves (with a
  *                row stride of hidden); needs residual
  *   normed       bf16 [num_rows, hidden] or NULL: y rounded once (for a router or a bf16 branch)
- * A row (block) that holds an infinity or a NaN gets a NaN scale and reads back as NaN throughout.
- * (as does a row of zeros under epsilon 0).
+ * A row (block) that holds an infinity or a NaN, or whose h does, gets a NaN scale and reads back as NaN throughout
+ * (as does a row of zeros under epsilon 0).  Finite rows are normed whatever their magnitude: one whose sum of squares
+ * leaves fp32 is scaled by a power of two first.
  * hidden % 8 == 0, hidden <= 32768, num_rows < 2^30; bf16 pointers 16-byte aligned.  Outputs must not overlap
  * inputs otherwise.
  * mi_ep_dequantize_rows reads them back: out = bf16(q * scale).
