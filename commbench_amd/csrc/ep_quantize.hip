@@ -103,13 +103,16 @@ __device__ __forceinline__ void store_codes(uint2* to, uint2 codes) {
                        __HIP_MEMORY_SCOPE_AGENT);
 }
 
+template <int kFormat>
+constexpr float kLargestCode = kFormat == kQuantInt8 ? 127.0f : 448.0f;
 // The scale of values whose largest magnitude has these bits.  Infinities and NaN order above every
 // finite value as integers, so a row (block) that holds one gets a NaN scale and reads back as NaN
-// throughout instead of as something finite.
+// throughout instead of as something finite.  A scale of zero, of values so small that the quotient vanishes too, is 1.
 template <int kFormat>
 __device__ __forceinline__ float scale_of(uint32_t amax_bits) {
   const float amax = __uint_as_float(amax_bits >= 0x7f800000u ? 0x7fc00000u : amax_bits);
-  return amax_bits == 0 ? 1.0f : amax / (kFormat == kQuantInt8 ? 127.0f : 448.0f);
+  const float scale = amax / kLargestCode<kFormat>;
+  return scale == 0.0f ? 1.0f : scale;
 }
 
 template <int kFormat>
@@ -126,7 +129,7 @@ __device__ __forceinline__ uint2 codes8(const float (&q)[8]) {
     out.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[7], b[6], 0x0c0c0400u), __builtin_amdgcn_perm(b[5], b[4], 0x0c0c0400u),
                                   0x05040100u);
   } else {
-    int lo = 0, hi = 0;  // the conversion rounds to nearest even; quotients end at 448 by construction
+    int lo = 0, hi = 0;  // the conversion rounds to nearest even; quotients end at 448
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
@@ -145,7 +148,12 @@ __device__ __forceinline__ uint2 quantize8(const float (&y)[8], const Divisor& d
     for (int i = 0; i < 8; ++i) q[i] = divide(y[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = y[i] / divide.scale;
+    for (int i = 0; i < 8; ++i) {
+      // A subnormal scale has few digits: its quotients may lie beyond the largest code (NaN passes the comparisons).
+      q[i] = y[i] / divide.scale;
+      if (q[i] > kLargestCode<kFormat>) q[i] = kLargestCode<kFormat>;
+      if (q[i] < -kLargestCode<kFormat>) q[i] = -kLargestCode<kFormat>;
+    }
   }
   return codes8<kFormat>(q);
 }

@@ -386,7 +386,7 @@ int mi_ep_combine(const void* y, int num_rows, const int* slot_map, const float*
  * Rows to 8 bits: what a dispatch sends when its payload is quantised, made where the row is made.
  *   h = x + residual;  y = h / sqrt(mean(h^2) + epsilon) * weight          (mi_ep_rms_norm_quantize)
  *   y = x                                                                  (mi_ep_quantize_rows)
- *   scale = max|y| / qmax, 1 where that is 0;  q = round(y / scale), ties to even
+ *   scale = max|y| / qmax, 1 where that is 0;  q = round(y / scale), ties to even, at most qmax
  * all in fp32 from the bf16 inputs, one rounding to the codes.
  *   format       MI_EP_QUANT_INT8_ROW: int8, qmax 127, one scale per row.
  *                MI_EP_QUANT_E4M3_BLOCK: e4m3 (the OCP form), qmax 448, one scale per 128 columns

@@ -1,4 +1,5 @@
-"""GPU tests of rms_norm_quantize at both ends of the value range: rows whose squares leave fp32.
+"""GPU tests of rms_norm_quantize at both ends of the value range: rows whose squares leave fp32, and rows so small that
+their scales are subnormal.
 
 NORM as in test_gpu_quantize_rows.py: 36 roundings of a norm's value relative to itself.  A row whose squares overflow or
 vanish is summed after a multiplication by a power of two, which rounds nothing but values 2^126 times smaller than the
@@ -10,6 +11,7 @@ import torch
 from commbench_amd import ops
 
 from . import expert_util as xu
+from . import gpu_util as gu
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +82,42 @@ def test_infinities_and_zeros_stay_what_they_are(width):
         assert torch.isnan(back[:2]).all()
         assert torch.isnan(back[2]).all() if eps == 0.0 else not back[2].any()
         assert torch.isfinite(back[3:]).all() and (back[3:].abs().amax(dim=1) > 1).all()
+
+
+# In units of 2^-149, the least fp32 value: 0 and 1 unit for the scale, quotients far beyond the codes, the last amounts
+# where a scale in whole units is coarse.
+UNITS = [1, 5, 63, 64, 100, 126, 127, 190, 191, 224, 225, 255, 380, 447, 508, 760, 1016, 3040, 6144, 12160, 16256, 32512, 65280]
+
+
+@pytest.mark.parametrize("width", [256, 1024, 4096, 7168, 16384])
+@pytest.mark.parametrize("quant", ["int8", "e4m3"])
+def test_codes_under_subnormal_scales(width, quant):
+    """y is a whole number of units to the bit: x = m * 2^-30 and weight 2^-119 under epsilon 1, beside which the mean of the
+    squares vanishes.  Scale, quotient and code are then single roundings; a quotient beyond the largest code is
+    that code, a scale that rounds to zero is 1."""
+    rng = np.random.default_rng(3)
+    rows = len(UNITS)
+    m = np.zeros((rows, width), dtype=np.float32)
+    for i, top in enumerate(UNITS):
+        step = max(1, top // 255 + (top % 255 > 0)) if top > 255 else 1
+        step = 1 << (step - 1).bit_length()                       # multiples of a power of two: 8 bits of bf16
+        m[i] = rng.integers(-(top // step), top // step + 1, width) * step
+        m[i, ::128], m[i, 1::128] = top // step * step, -(top // step * step)
+    x = torch.from_numpy(m * np.float32(2.0 ** -30)).to(torch.bfloat16)
+    assert np.array_equal(x.to(torch.float32).numpy(), m * np.float32(2.0 ** -30))
+    assert float((np.float64(m) ** 2).mean(axis=1).max()) * 2.0 ** -60 < 2.0 ** -25       # lost beside epsilon
+    g = torch.full((width,), 2.0 ** -119, dtype=torch.bfloat16, device=xu.DEV)
+    q, s = ops.rms_norm_quantize(x.to(xu.DEV), g, 1.0, quant=quant)
+    y = m * np.float32(2.0 ** -149)
+    top = np.float32(127.0 if quant == "int8" else 448.0)
+    blocks = y.reshape(rows, -1, width if quant == "int8" else 128)
+    scales = (np.abs(blocks).max(axis=2) / top).astype(np.float32)
+    scales[scales == 0] = 1.0
+    np.testing.assert_array_equal(s.cpu().numpy(), scales)
+    quotients = np.clip(blocks / scales[:, :, None], -top, top).astype(np.float32).reshape(rows, width)
+    if quant == "int8":
+        np.testing.assert_array_equal(q.cpu().numpy(), np.rint(quotients).astype(np.int8))
+    else:
+        want = torch.from_numpy(quotients).to(torch.float8_e4m3fn)
+        np.testing.assert_array_equal(xu.f64(q), xu.f64(want))
+    assert gu.bf16_bits(ops.dequantize_rows(q, s)).shape == (rows, width)
