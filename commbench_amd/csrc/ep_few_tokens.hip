@@ -69,11 +69,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* base, int 
 }
 __device__ __forceinline__ void wait_lds_and_meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// silu(g) * u as the sum of two bf16 values.
+// silu(g) * u as the sum of two bf16 values.  A finite product that bf16 would round to infinity has the largest finite
+// bf16 as its first (its bits are those of the infinity less one); the rest of an infinity or a NaN is none.
 __device__ __forceinline__ void activate(float g, float u, uint32_t& high, uint32_t& low) {
   const float act = g / (1.0f + __expf(-g)) * u;
+  const bool finite = __builtin_isfinite(act);
   high = f32_to_bf16_bits(act);
-  low = __builtin_isfinite(act) ? f32_to_bf16_bits(act - bf16_lo(high)) : 0;  // the rest of an infinity is none
+  if (finite && (high & 0x7fffu) == 0x7f80u) --high;
+  low = finite ? f32_to_bf16_bits(act - bf16_lo(high)) : 0;
 }
 
 // Who meets whom, made by every workgroup for itself from the ids: `entries` lists the met experts by their
