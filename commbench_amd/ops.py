@@ -740,7 +740,7 @@ def moe_few_tokens(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: Option
         for w, name in ((w13, "w13"), (w2, "w2")):
             _require(w.dtype == torch.bfloat16 and w.is_contiguous() and w.device == dev and w.data_ptr() % 16 == 0,
                      f"{name} must be contiguous bf16 (or int8 with scales) on the device of x")
-    bias_0, bias_1 = bias if isinstance(bias, tuple) else (bias, None)
+    bias_0, bias_1 = (bias, None) if bias is None or isinstance(bias, torch.Tensor) else bias
     for b in (bias_0, bias_1):
         _require(b is None or (b.dtype == torch.bfloat16 and b.is_contiguous() and tuple(b.shape) == (T, H)
                                and b.device == dev and b.data_ptr() % 16 == 0),
