@@ -42,6 +42,7 @@ SILU_MUL = 1           # MI_EP_MATMUL_SILU_MUL
 QUANT_BLOCK = 128      # MI_EP_QUANT_BLOCK: columns that share an e4m3 scale
 QUANT_MAX_HIDDEN = 32768
 FEW_MAX_ROUTES = 1024  # MI_EP_FEW_MAX_ROUTES
+FLOAT32_MAX = torch.finfo(torch.float32).max
 _QUANT_FORMATS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _SCHEDULE_FLAGS = {"auto": 0, "token": BY_TOKEN, "destination": BY_DESTINATION}
 
@@ -593,7 +594,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     g_at = weight.data_ptr()
     _require(weight.dtype is torch.bfloat16 and weight.shape == (H,) and weight.is_contiguous() and weight.device == dev
              and g_at % 16 == 0, "weight must be contiguous bf16 [hidden] on the device of x")
-    _require(0.0 <= eps < float("inf"), "eps must be finite and not negative")
+    _require(0.0 <= eps <= FLOAT32_MAX, "eps must be finite in float32 and not negative")
     out_residual = r_at = out_at = None
     r_stride = 0
     if residual is not None:

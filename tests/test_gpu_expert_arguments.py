@@ -21,3 +21,10 @@ def test_biases_in_a_list_as_combine_takes_them():
         assert torch.equal(few(list(pair)), few(pair))
     y, slots = x, torch.arange(T, dtype=torch.int32, device=xu.DEV).view(T, 1)
     assert torch.equal(ops.combine(y, slots, bias=[b0, b1]), ops.combine(y, slots, bias=(b0, b1)))
+
+
+@pytest.mark.parametrize("eps", [float("nan"), float("inf"), -1e-6, 1e39, 3.5e38])
+def test_an_epsilon_that_fp32_cannot_hold_is_refused(eps):
+    x = torch.ones((2, 64), dtype=torch.bfloat16, device=xu.DEV)
+    with pytest.raises(ValueError, match="eps must be"):
+        ops.rms_norm_quantize(x, torch.ones(64, dtype=torch.bfloat16, device=xu.DEV), eps)
