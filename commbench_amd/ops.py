@@ -290,6 +290,13 @@ class Buffer:
         _require(w13.dim() == 3 and w2.dim() == 3 and w13.shape[0] == self.num_experts and w2.shape[0] == self.num_experts
                  and w13.shape[1] == 2 * w2.shape[2] and w2.shape[1] == w13.shape[2] == q.shape[1],
                  "w13 must be [experts, 2 * intermediate, hidden] and w2 [experts, hidden, intermediate]")
+        dev = self.workspace.device
+        biases = bias if isinstance(bias, (tuple, list)) else (bias,)
+        _require(all(t is None or t.device == dev for t in (q, scales, topk_idx, topk_weights, *biases)),
+                 "q, scales, topk_idx, topk_weights and bias must be on the buffer's device")
+        if dev.index != torch.cuda.current_device():   # dispatch and combine take the current device's stream
+            with torch.cuda.device(dev):
+                return self.moe_int8(q, scales, topk_idx, topk_weights, w13, w13_scales, w2, w2_scales, bias, expert_alignment)
         if q.shape[0] == 0:
             return torch.empty((0, q.shape[1]), dtype=torch.bfloat16, device=q.device)
         recv, recv_scales, _, h = self.dispatch(q, scales, topk_idx, topk_weights, expert_alignment)
