@@ -13,7 +13,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "ep_device.h"
+#include "ep_expert.h"
 #include "ep_stage.h"
 
 namespace mi_ep {

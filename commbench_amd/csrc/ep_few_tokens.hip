@@ -13,7 +13,7 @@
 // slots of a token are added in ascending order at the end.
 #include <atomic>
 
-#include "ep_device.h"
+#include "ep_expert.h"
 #include "ep_stage.h"
 
 namespace mi_ep {

@@ -11,7 +11,7 @@
 // fp32 at either end is brought near one by a power of two, from the registers, and summed again.  Bound by HBM: 7
 // bytes an element move (x, residual in, residual out, q) for about 25 vector instructions per 8 elements
 // and reduction step.
-#include "ep_device.h"
+#include "ep_expert.h"
 
 namespace mi_ep {
 namespace {

@@ -1,6 +1,6 @@
 // Stages of rows in LDS, filled by loads that bypass the registers, for gfx950.
 #pragma once
-#include "ep_device.h"
+#include "ep_expert.h"
 
 namespace mi_ep {
 
