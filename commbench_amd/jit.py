@@ -22,7 +22,6 @@ import ctypes
 import hashlib
 import os
 import shutil
-import subprocess
 from typing import Dict, Optional
 
 from . import _lib
@@ -98,8 +97,22 @@ def library_path(**shapes: int) -> str:
     return os.path.join(cache_dir(), f"libmi_ep_{h.hexdigest()[:16]}.so")
 
 
+def _object_path(name: str, files: Dict[str, str]) -> Optional[str]:
+    """Where the object of a source that holds no fixed shape lives in the cache, whatever the shapes; None for a source
+    that is compiled for every set of them.  An overlay's source may use the shapes, and so may its headers."""
+    shipped = [os.path.join(hip_build.CSRC_DIR, n) for n in [name] + HEADERS]
+    if name not in hip_build.SHAPE_FREE_SOURCES or [files[n] for n in [name] + HEADERS] != shipped:
+        return None
+    h = hashlib.sha256(" ".join(hip_build.HIPCC_FLAGS).encode())
+    for path in shipped + [os.path.join(ROOT, "include", "mi_ep.h")]:
+        with open(path, "rb") as f:
+            h.update(f.read())
+    return os.path.join(cache_dir(), f"{os.path.splitext(name)[0]}_{h.hexdigest()[:16]}.o")
+
+
 def compile_library(**shapes: int) -> str:
-    """Compiles (or finds in the cache) the library with the given shapes fixed; returns its path."""
+    """Compiles (or finds in the cache) the library with the given shapes fixed; returns its path.  The objects of
+    the sources that hold no shape stay in the cache for the libraries of other shapes."""
     out = library_path(**shapes)
     if os.path.exists(out):
         return out
@@ -111,15 +124,31 @@ def compile_library(**shapes: int) -> str:
     os.makedirs(csrc)
     os.makedirs(os.path.join(stage, "include"))
     shutil.copy(os.path.join(ROOT, "include", "mi_ep.h"), os.path.join(stage, "include", "mi_ep.h"))
-    for name, path in source_files().items():
+    files = source_files()
+    for name, path in files.items():
         shutil.copy(path, os.path.join(csrc, name))
-    cmd = [_hipcc(), *hip_build.HIPCC_FLAGS, *[f"-D{k}={v}" for k, v in _defines(shapes).items()],
-           "-o", f"{out}.{os.getpid()}.tmp"] + [os.path.join(csrc, s) for s in hip_build.SOURCES]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    shutil.rmtree(stage, ignore_errors=True)
-    if proc.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + proc.stdout + proc.stderr)
-    os.replace(f"{out}.{os.getpid()}.tmp", out)     # atomic: a reader sees the old file or the whole new one
+    defines = [f"-D{k}={v}" for k, v in _defines(shapes).items()]
+    try:
+        objects, missing = [], {}
+        for name in hip_build.SOURCES:
+            cached = _object_path(name, files)
+            if cached is None or not os.path.exists(cached):
+                staged = os.path.join(stage, name + ".o")
+                missing[staged] = [os.path.join(csrc, name)] + (defines if cached is None else [])
+                objects.append(staged)
+            else:
+                objects.append(cached)
+        hip_build.compile_objects(_hipcc(), missing)
+        linked = os.path.join(stage, "linked.so")
+        hip_build.link_library(_hipcc(), linked, objects)
+        # Atomic: a reader sees the old file or the whole new one.
+        for staged in missing:
+            cached = _object_path(os.path.basename(staged)[:-2], files)
+            if cached is not None:
+                os.replace(staged, cached)
+        os.replace(linked, out)
+    finally:
+        shutil.rmtree(stage, ignore_errors=True)
     return out
 
 
