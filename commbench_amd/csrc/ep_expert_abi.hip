@@ -31,6 +31,15 @@ inline bool scales_distinct(int num_rows, int hidden, int format, long long row_
   return row_stride >= (groups - 1) * hidden_stride + 1 || hidden_stride >= (num_rows - 1) * row_stride + 1;
 }
 inline bool row_stride_ok(long long stride, int hidden) { return stride >= hidden && stride % 8 == 0; }
+// Whether written rows, one behind the other, lie across others' rows of the same width: a workgroup would write what
+// another one has yet to read.  The same rows (in place) do not.
+inline bool written_across(const void* written, const void* read, long long read_stride, int num_rows, int hidden) {
+  const long long out = reinterpret_cast<long long>(written), in = reinterpret_cast<long long>(read);
+  const long long width = 2LL * hidden, stride = 2 * read_stride;
+  if (num_rows == 0 || (out == in && stride == width)) return false;
+  const long long first = in + width > out ? 0 : (out - in - width) / stride + 1;  // the first row that ends behind `out`
+  return first < num_rows && in + first * stride < out + num_rows * width;
+}
 
 inline bool few_tokens_shape_ok(int num_tokens, int num_topk) {
   return num_tokens >= 0 && num_topk > 0 && num_topk <= MI_EP_MAX_TOPK &&
@@ -53,9 +62,8 @@ int mi_ep_rms_norm_quantize(const void* x, long long x_row_stride, const void* r
   if (!row_stride_ok(x_row_stride, hidden) || (residual != nullptr && !row_stride_ok(residual_row_stride, hidden)))
     return MI_EP_EINVAL;
   if (residual_out != nullptr && residual == nullptr) return MI_EP_EINVAL;
-  // In place only where the output's rows lie on the input's.
-  if (residual_out != nullptr && ((residual_out == x && x_row_stride != hidden) ||
-                                  (residual_out == residual && residual_row_stride != hidden)))
+  if (residual_out != nullptr && (written_across(residual_out, x, x_row_stride, num_rows, hidden) ||
+                                  written_across(residual_out, residual, residual_row_stride, num_rows, hidden)))
     return MI_EP_EINVAL;
   if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(residual_out) || !aligned16(normed) ||
       !aligned8(q))

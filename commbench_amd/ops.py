@@ -594,7 +594,8 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     `quant` is "int8" (a scale for each row, max|y| / 127) or "e4m3" (float8_e4m3fn, a scale for each 128
     columns, max|y| / 448); scales come as float32 [rows, groups], what dispatch takes.  Returns (q, scales),
     then the new residual stream bf16(h) when `residual` is given (written over it with
-    `update_residual`), then bf16(y) with `normed`.  x and residual may be views with padded rows."""
+    `update_residual`, which refuses an x that lies across its rows), then bf16(y) with `normed`.  x and residual may be views
+    with padded rows."""
     T, H, x_stride, x_at = _check_rows(x, "x")
     fmt, dtype, groups = _quant_format(quant, H)
     dev = x.device

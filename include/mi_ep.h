@@ -402,7 +402,7 @@ int mi_ep_combine(const void* y, int num_rows, const int* slot_map, const float*
  *   scales       float, element j of row r at scales[r * scales_row_stride + j * scales_hidden_stride],
  *                the strides mi_ep_dispatch_strided_scales takes; written scales may not share a place
  *   residual_out bf16 [num_rows, hidden] or NULL: h rounded once.  It may be residual or x themselves (with a
- *                row stride of hidden); needs residual
+ *                row stride of hidden), but not lie across their rows (refused); needs residual
  *   normed       bf16 [num_rows, hidden] or NULL: y rounded once (for a router or a bf16 branch)
  * A row (block) that holds an infinity or a NaN, or whose h does, gets a NaN scale and reads back as NaN throughout
  * (as does a row of zeros under epsilon 0).  Finite rows are normed whatever their magnitude: one whose sum of squares
