@@ -7,9 +7,10 @@
 //
 // What bounds it depends on the rows of an expert.  Few rows: reading the weights once (256 experts x 4096 x 7168 with 2 rows
 // each 1071 us, 7.0 TB/s; with 32 rows 1126).  Hundreds: the matrix units at the clock that the card's power limit leaves
-// them (8192^3 442 us, 2490 TOP/s, clock near 1.6 GHz), less what ragged heights leave empty: a segment is computed in
-// blocks of 64 rows (8192 tokens' 65536 rows over 256 experts x 4096 x 7168: 2390 us, of which the empty part of the
-// blocks is an eighth).
+// them (8192^3 442 to 474 us by card, 2490 to 2320 TOP/s, clock near 1.6 GHz), less what ragged heights leave empty: a segment is
+// computed in blocks of 64 rows (8192 tokens' 65536 rows over 256 experts x 4096 x 7168: 2390 to 2450 us, of which the empty
+// part of the blocks is an eighth; the matrix units are busy for 46 % of it at 1.8 GHz, since weights that nobody has read
+// before are asked for about one stage, 1 us, ahead).
 #include <atomic>
 #include <type_traits>
 
@@ -183,6 +184,7 @@ __global__ __launch_bounds__(kSmallThreads) void ep_expert_matmul_small_kernel(c
 // ---- large tiles: up to 256 rows by 256 channels ----------------------------------------------------------
 // One persistent workgroup a compute unit, four waves of 128 x 128: a stage's 64 KiB give 128 products of 32 x 32 x 32, half
 // a fragment read from LDS for each, and the accumulators fill the 256 registers that the products can add to directly.
+// The rest does not quite fit: 4 vector registers and 178 (silu 243) scalar ones are spilled.
 // With loads of 128 bytes a row (64: a sixth slower), LDS rows permuted so that no bank is met twice, reads and loads spread
 // between the products one by one, and the next tile's loads and this tile's stores on their way at once.
 // Rejected: 320-row tiles (the accumulators no longer fit beside the fragments and are copied about), tiles claimed from

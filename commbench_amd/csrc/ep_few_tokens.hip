@@ -2,9 +2,11 @@
 //   act[r, i] = silu(Wg[e] x[t])[i] * (Wu[e] x[t])[i]                     r = route (t, k) to expert e
 //   out[t, :] = sum_k w[t, k] * W2[e_k] act[(t, k), :] (+ biases)
 // With a few tokens every expert sees one or a handful of rows, so the time is that of reading the met
-// experts' weights once; moving rows to the experts and back would only add launches.  48 tokens of top 8 over 256
-// experts, 7168 x 2048 int8, read 8.7 GB in 1329 us (6.5 TB/s), 16 tokens over 128 experts, 4096 x 1408 bf16, 2.9 GB
-// in 529 us; one token's 352 MB take 75 us, where starting and draining two kernels shows.  Weights are
+// experts' weights once; moving rows to the experts and back would only add launches.  By card, 48 tokens of top 8 over 256
+// experts, 7168 x 2048 int8, read 8.7 GB in 1330 to 1410 us (6.2 to 6.5 TB/s), 16 tokens over 128 experts, 4096 x 1408 bf16,
+// 2.9 GB in 450 to 530 us; one token's 352 MB take 72 to 75 us, where starting and draining two kernels shows.  128 tokens of the
+// first take 1890 us (11.1 GB, 5.9 TB/s).  Where experts get many routes it is far from that: 128 tokens of top 8 over 64
+// experts, 4096 x 1536 int8, 587 us for 1.2 GB.  Weights are
 // bf16, or int8 with a scale for each output channel (widened to bf16 in registers, exactly), products
 // run on the matrix units with the weights as the 16-row operand and up to 16 of an expert's routes as
 // the columns, sums are fp32.  act is kept as the sum of two bf16 values (16 bits: one alone would be as large an
@@ -699,6 +701,8 @@ hipError_t launch_tiles(const FewTokensArgs& a, int compute_units, hipStream_t s
     if (e != hipSuccess) return e;
     lds_limit_raised[ordinal].store(1, std::memory_order_release);
   }
+  // Two workgroups a compute unit; the second product's have room for each other up to 853 routes.  Beyond, the grid's second half
+  // follows the first (106 tokens of top 8 over 256 experts, 7168 x 2048, 1768 us, 107 tokens 1869).
   hipLaunchKernelGGL((ep_few_tokens_tiles_kernel<kInt8, kDown>), dim3(static_cast<unsigned>(2 * compute_units)),
                      dim3(kFirstThreads), lds, stream, a);
   return hipGetLastError();
@@ -733,7 +737,9 @@ hipError_t launch_down(const FewTokensArgs& a, hipStream_t stream) {
 
 template <bool kInt8>
 hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
-  // Columns of a pass by the routes that an expert gets on average: every further pass reads its weights again.
+  // Columns of a pass by the routes that an expert gets on average: every further pass reads its weights again.  Four
+  // blocks of 16 columns leave no registers for loads further ahead (with int8 weights 32 are spilled): 128 tokens of top 8
+  // over 64 experts, 4096 x 1536, read their weights at 2 TB/s.
   const int routes = a.num_tokens * a.num_topk;
   const bool many = routes > 8 * a.num_experts;
   DeviceTraits dev{};
@@ -751,8 +757,8 @@ hipError_t launch_few_tokens_with(const FewTokensArgs& a, hipStream_t stream) {
       : tiles(a.hidden, a.intermediate, kSetRows, 4) ? launch_tiles<kInt8, false>(a, dev.compute_units, stream)
                                                   : launch_gate_up<kInt8, 1, 2>(a, stream);
   if (e != hipSuccess) return e;
-  // The second product's tiles cost a launch and the traffic of y: 48 tokens (14336 items) 1407 / 1329, 16 tokens (4096) 529 /
-  // 531, 12 tokens (1536) 115 / 122.
+  // The second product's tiles cost a launch and the traffic of y, and pay by the items: 48 tokens (14336 items) 1407 / 1329,
+  // 16 tokens (4096) 529 / 531, which is where they begin to, 12 tokens (1536) 115 / 122.
   if (tiles(a.intermediate, a.hidden, 2 * kSetRows, 16)) {
     e = launch_tiles<kInt8, true>(a, dev.compute_units, stream);
     if (e != hipSuccess) return e;

@@ -345,7 +345,8 @@ hipError_t launch_quantize_as(const QuantizeArgs& args, hipStream_t stream) {
   const auto wide_rows = [&](auto kernel, int threads) { in_pieces(kernel, 1 << 21, threads, 1); };
   const QuantizeArgs& a = args;
   // With fewer rows than compute units the latency of one row is the time: more threads to a row, fewer vectors each
-  // (16 rows of 7168 columns: 6.6 us with 256 threads of four vectors, 4.8 us with 1024 of one).
+  // (16 rows of 7168 columns: 6.6 us with 256 threads of four vectors, 4.8 us with 1024 of one).  Measured and taken for these
+  // widths only: 16 rows of 4096, a wave each, take 7.5 us.
   if (a.num_rows <= 256 && a.row_vecs > 512 && a.row_vecs <= 1024) wide_rows(&ep_quantize_rows_kernel<1024, 1, kNorm, kFormat>, 1024);
   else if (a.row_vecs <= 64) wave_rows(&ep_quantize_rows_kernel<64, 1, kNorm, kFormat>);
   else if (a.row_vecs <= 128) wave_rows(&ep_quantize_rows_kernel<64, 2, kNorm, kFormat>);

@@ -284,7 +284,10 @@ class Buffer:
         """The whole expert layer on an int8 payload (rms_norm_quantize): dispatch, gate and up product with
         silu(gate) * up, requantisation, down product, weighted combine (+ biases).  Weights as in
         grouped_matmul_int8: w13 [experts, 2 * intermediate, hidden] (gate rows, then up rows), w2 [experts,
-        hidden, intermediate].  For a handful of tokens moe_few_tokens is the faster way."""
+        hidden, intermediate].  Between the products the activation is rounded to bf16 and then to int8 with a scale for each
+        row; products that leave bf16's range make their row NaN.  For a handful of tokens moe_few_tokens is as fast or
+        faster (over 256 experts of 7168 x 2048 up to about 16 tokens, over 64 of 4096 x 1536 up to about 32), and more exact.
+        All tensors are on the buffer's device; calls on one Buffer must not overlap in time."""
         _require(q.dtype == torch.int8, "q must be int8 (rms_norm_quantize or quantize_rows)")
         _require(scales is not None and scales.dim() == 2 and scales.shape[1] == 1, "scales must be float32 [num_tokens, 1]")
         _require(w13.dim() == 3 and w2.dim() == 3 and w13.shape[0] == self.num_experts and w2.shape[0] == self.num_experts
@@ -720,7 +723,10 @@ def moe_few_tokens(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: Option
     x is bf16 [tokens, hidden]; w13 [experts, 2 * intermediate, hidden] holds the gate rows, then the up
     rows, w2 is [experts, hidden, intermediate]; both bf16, or int8 with float32 scales [experts, rows].
     topk_idx, topk_weights (None: a plain sum) and bias as in dispatch and combine; a token whose slots are all
-    masked gets its biases.  With many tokens Buffer.moe_int8 is the faster way."""
+    masked gets its biases.  The activation between the two products is carried in 16 bits of mantissa, everything else in fp32;
+    int8 codes are summed before their scale is applied.  Weights have to be finite.  With int8 weights and more than about
+    16 tokens (over 256 experts of 7168 x 2048; 32 over 64 of 4096 x 1536) Buffer.moe_int8 is the faster way, at the
+    price of int8 activations."""
     _require(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0,
              "x must be a contiguous bf16 [num_tokens, hidden] GPU tensor")
     dev = x.device

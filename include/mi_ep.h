@@ -454,8 +454,9 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
  * The whole expert layer for a few tokens, in two or three launches and without moving a row:
  *   combined_x[t] = bf16( sum_k w[t,k] * W2[e] (silu(Wgate[e] x[t]) * (Wup[e] x[t])) + bias_0[t] + bias_1[t] ),
  *   e = topk_idx[t, k]; slots outside [0, num_experts) are no routes, a token without routes gets its biases
- * (zeros without).  It reads the weights of the experts that the tokens met, once; with many tokens dispatch, the
- * products above and combine are the faster way.
+ * (zeros without).  It reads the weights of the experts that the tokens met, once (again for every 16 routes of an expert,
+ * 64 where there are more than eight an expert); with many tokens dispatch, the products above and combine are the
+ * faster way.
  *   x            bf16 [num_tokens, hidden]
  *   w13, w2      [num_experts, 2 * intermediate, hidden] (gate rows, then up rows), [num_experts, hidden,
  *                intermediate]: bf16 with both scales NULL, or int8 with w13_scales float [num_experts, 2 *
@@ -463,8 +464,9 @@ int mi_ep_grouped_matmul_int8(const void* a, const float* a_scales, long long a_
  *   topk_weights float [num_tokens, num_topk] or NULL: a plain sum
  *   workspace    mi_ep_moe_few_tokens_workspace_bytes bytes, 16-byte aligned, no initialisation; calls that
  *                share one must not overlap in time
- * Sums are fp32 in an order that depends on the shapes alone; the activation between the two products is
- * carried in 16 bits of mantissa.  num_tokens * num_topk <= MI_EP_FEW_MAX_ROUTES; hidden % 16 == 0, intermediate % 16 == 0, both
+ * Sums are fp32 in an order that depends on the shapes alone (int8 codes are summed before their scale is applied); the
+ * activation between the two products is carried in 16 bits of mantissa, as two bf16 values, so weights have to be finite: an
+ * infinite one of w2 gives NaN where the second value is zero.  num_tokens * num_topk <= MI_EP_FEW_MAX_ROUTES; hidden % 16 == 0, intermediate % 16 == 0, both
  * at most 65536; x, w13, w2, biases and combined_x 16-byte aligned.
  */
 #define MI_EP_FEW_MAX_ROUTES 1024
