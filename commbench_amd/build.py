@@ -29,7 +29,7 @@ def _run(cmd: Sequence[str]) -> str:
 def compile_objects(hipcc: str, objects: Dict[str, Sequence[str]]) -> str:
     """Compiles several sources at once: {object file: [source, further flags]}.  Returns what the compiler said."""
     flags = [flag for flag in HIPCC_FLAGS if flag != "-shared"]
-    jobs = min(len(objects), int(os.environ.get("MAX_JOBS", 0)) or os.cpu_count() or 1)
+    jobs = min(len(objects), int(os.environ.get("MAX_JOBS") or 0) or os.cpu_count() or 1)
     with ThreadPoolExecutor(max(jobs, 1)) as pool:
         said = pool.map(lambda item: _run([hipcc, *flags, *item[1][1:], "-c", "-o", item[0], item[1][0]]), objects.items())
         return "".join(said)

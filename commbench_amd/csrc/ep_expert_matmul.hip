@@ -11,10 +11,10 @@
 // computed in blocks of 64 rows (8192 tokens' 65536 rows over 256 experts x 4096 x 7168: 2390 to 2450 us, of which the empty
 // part of the blocks is an eighth; the matrix units are busy for 46 % of it at 1.8 GHz, since weights that nobody has read
 // before are asked for about one stage, 1 us, ahead).
-#include <atomic>
 #include <type_traits>
 
 #include "ep_expert.h"
+#include "ep_launch.h"
 #include "ep_stage.h"
 
 namespace mi_ep {
@@ -634,22 +634,13 @@ hipError_t launch_expert_matmul(const ExpertMatmulArgs& a, hipStream_t stream) {
   const bool big = a.num_rows > 12LL * a.num_experts && big_tiles >= 96;
   if (big) {
     DeviceTraits dev{};
-    int ordinal = 0;
     hipError_t err = device_traits(stream, &dev);
-    if (err == hipSuccess) err = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
     if (err != hipSuccess) return err;
-    // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
-    constexpr int kMaxDevices = 64;
-    static std::atomic<int> lds_limit_raised[2][kMaxDevices];
-    if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
-    std::atomic<int>& raised = lds_limit_raised[a.silu_mul ? 1 : 0][ordinal];
-    if (raised.load(std::memory_order_acquire) == 0) {
-      const void* kernel = a.silu_mul ? reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<true>)
-                                      : reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<false>);
-      err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBigLds);
-      if (err != hipSuccess) return err;
-      raised.store(1, std::memory_order_release);
-    }
+    static LdsCeiling ceilings[2];
+    const void* kernel = a.silu_mul ? reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<true>)
+                                    : reinterpret_cast<const void*>(&ep_expert_matmul_big_kernel<false>);
+    err = ceilings[a.silu_mul ? 1 : 0].raise(kernel, kBigLds, stream);
+    if (err != hipSuccess) return err;
     const dim3 grid(static_cast<unsigned>(dev.compute_units));
     if (a.silu_mul)
       hipLaunchKernelGGL((ep_expert_matmul_big_kernel<true>), grid, dim3(kBigThreads), kBigLds, stream, a);

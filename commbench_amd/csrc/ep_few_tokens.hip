@@ -13,9 +13,8 @@
 // error as the rounding of the result), which the second product takes as two columns.
 // A sum never depends on the order in which waves finish: each (route, output) has one writer, and the
 // slots of a token are added in ascending order at the end.
-#include <atomic>
-
 #include "ep_expert.h"
+#include "ep_launch.h"
 #include "ep_stage.h"
 
 namespace mi_ep {
@@ -688,19 +687,10 @@ hipError_t launch_gate_up(const FewTokensArgs& a, hipStream_t stream) {
 template <bool kInt8, bool kDown>
 hipError_t launch_tiles(const FewTokensArgs& a, int compute_units, hipStream_t stream) {
   const int lds = kTileMeetingAt<kDown> + static_cast<int>(Meeting<16>::bytes(a.num_tokens * a.num_topk));
-  int ordinal = 0;
-  hipError_t e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
+  static LdsCeiling ceiling;
+  const hipError_t e =
+      ceiling.raise(reinterpret_cast<const void*>(&ep_few_tokens_tiles_kernel<kInt8, kDown>), 96 * 1024, stream);
   if (e != hipSuccess) return e;
-  // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
-  constexpr int kMaxDevices = 64;
-  static std::atomic<int> lds_limit_raised[kMaxDevices];
-  if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
-  if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_tiles_kernel<kInt8, kDown>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
-    if (e != hipSuccess) return e;
-    lds_limit_raised[ordinal].store(1, std::memory_order_release);
-  }
   // Two workgroups a compute unit; the second product's have room for each other up to 853 routes.  Beyond, the grid's second half
   // follows the first (106 tokens of top 8 over 256 experts, 7168 x 2048, 1768 us, 107 tokens 1869).
   hipLaunchKernelGGL((ep_few_tokens_tiles_kernel<kInt8, kDown>), dim3(static_cast<unsigned>(2 * compute_units)),
@@ -716,19 +706,10 @@ hipError_t launch_down(const FewTokensArgs& a, hipStream_t stream) {
   const size_t scratch = static_cast<size_t>(a.num_experts) * 2 * sizeof(int);
   const size_t lds = Meeting<1>::bytes(routes) + (sums > scratch ? sums : scratch);
   if (lds > 60 * 1024) {
-    // The kernel's LDS ceiling is raised once per device; the flags only ever go from 0 to 1.
-    int ordinal = 0;
-    hipError_t e = stream != nullptr ? hipStreamGetDevice(stream, &ordinal) : hipGetDevice(&ordinal);
+    static LdsCeiling ceiling;
+    const hipError_t e =
+        ceiling.raise(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kBlocks, kDepth, kFold>), 80 * 1024, stream);
     if (e != hipSuccess) return e;
-    constexpr int kMaxDevices = 64;
-    static std::atomic<int> lds_limit_raised[kMaxDevices];
-    if (ordinal < 0 || ordinal >= kMaxDevices) return hipErrorInvalidDevice;
-    if (lds_limit_raised[ordinal].load(std::memory_order_acquire) == 0) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&ep_few_tokens_down_kernel<kInt8, kBlocks, kDepth, kFold>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
-      if (e != hipSuccess) return e;
-      lds_limit_raised[ordinal].store(1, std::memory_order_release);
-    }
   }
   hipLaunchKernelGGL((ep_few_tokens_down_kernel<kInt8, kBlocks, kDepth, kFold>), dim3(static_cast<unsigned>(a.hidden / 16)),
                      dim3(kSecondThreads), lds, stream, a, splits);

@@ -29,7 +29,7 @@ from . import build as hip_build
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
-HEADERS = ["ep_device.h", "ep_expert.h", "ep_stage.h"]
+HEADERS = ["ep_device.h", "ep_expert.h", "ep_launch.h", "ep_stage.h"]
 SHAPE_MACROS = {
     "num_topk": "MI_EP_FIXED_TOPK",
     "num_experts": "MI_EP_FIXED_EXPERTS",
@@ -46,7 +46,7 @@ def init_jit(overlay_root: Optional[str] = None, rocm_home: Optional[str] = None
     """Sets where later compilations take their sources and compiler from.  A file of
     `overlay_root` named like a shipped kernel source (ep_layout.hip, ep_permute.hip, ep_combine.hip,
     ep_abi.hip, ep_host.hip, ep_expert_abi.hip, ep_quantize.hip, ep_expert_matmul.hip, ep_few_tokens.hip, ep_device.h,
-    ep_expert.h, ep_stage.h) replaces it, as the reference's overlay replaces one header; `rocm_home` is the toolchain root (hipcc
+    ep_expert.h, ep_launch.h, ep_stage.h) replaces it, as the reference's overlay replaces one header; `rocm_home` is the toolchain root (hipcc
     under bin/).  The quantisation and expert kernels hold no fixed shape: a library built for
     one takes every shape in those calls."""
     if overlay_root is not None and not os.path.isdir(overlay_root):
